@@ -172,6 +172,40 @@ int lcq_silu_mul(const void* gate, const void* up, void* out, int64_t n, int dty
 int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
 
 /*
+ * The int8 path: products of int8 tokens and int8 weights, with a scale for each token and each output channel.  No
+ * counterpart in the reference, whose int8 matvec keeps float activations.
+ *
+ * lcq_int8_matmul: out[m, n] = (sum_k x[m, k] * w[n, k]) * x_scales[m] * w_scales[n].
+ *   x int8 [M, K] with rows ldx bytes apart, x_scales float32 [M]; w int8 [N, K] with rows ldw bytes apart, w_scales [N] of
+ *   w_scale_dtype (lcq_quantize_int8 with group_size = K makes both); out [M, N] of out_dtype, contiguous.  The sum is an exact
+ *   int32 (K <= 131071, else LCQ_ERR_UNSUPPORTED), the scales are applied in float32, the result is rounded once.  Rows on 16 bytes
+ *   (x, w, ldx, ldw multiples of 16) are read by TMA; any other are fetched by slower loads.
+ *   workspace: as for lcq_matmul_int4, of lcq_int8_matmul_workspace_bytes() bytes; the same buffer may serve both.  Nothing is read
+ *   before the kernel ahead on the stream has completed: unlike lcq_matmul_int4, weights may be written by it.
+ *
+ * lcq_quantize_tokens: q[r, :] = rint(v / s), scales[r] = s = max|v| / 127 with v = x[r, :] or, where `weight` is given,
+ *   rms_norm(x[r, :]) as in lcq_rms_norm.  A row of zeros has s = 1; s is at least 2^-126; a row that holds an infinity or a NaN gets
+ *   s = NaN and q = 0, so that every product with it is NaN.  Without `weight` the results are those of lcq_quantize_int8 (style 0, group_size = n).
+ *   x of `dtype`, rows ldx elements apart; q int8, rows ldq bytes apart (multiples of 16 suit lcq_int8_matmul); scales float32 [rows].
+ * lcq_silu_mul_tokens: the same of v = gate * sigmoid(gate) * up; gate and up may be halves of the rows of one matrix.
+ * lcq_residual_norms: what stands between two blocks, in one pass:
+ *     y = delta, or rms_norm(delta) * post_weight;  y *= gate row r / (rows / gate_rows);  hidden_out = hidden + scale * y, rounded to `dtype`;
+ *     out = rms_norm(hidden_out) * weight, of `dtype`, or (scales given) as int8 tokens.
+ *   post_weight and gate may be NULL; weight NULL: no norm follows, out is not written.  gate: [gate_rows, n], rows % gate_rows == 0.
+ *   hidden, delta, hidden_out [rows, n], contiguous; hidden_out may be hidden, and out (not int8) may be delta.
+ */
+int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, void* out,
+                    int M, int N, int K, int w_scale_dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K);
+int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q, int64_t ldq, void* scales, int64_t rows, int n,
+                        float eps, int dtype, void* stream);
+int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* q, int64_t ldq, void* scales,
+                        int64_t rows, int n, int dtype, void* stream);
+int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
+                       const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n, float eps,
+                       int dtype, void* stream);
+
+/*
  * Embedding lookup: out[t, :] = table[token_ids[t], :]; token_ids int32 [tokens], table [vocab, dim],
  * out [tokens, dim], both of `dtype`.  Replaces `_embed_fp32` / `_embed_fp16`
  * (locomp/_builtin_kernels.py:8-25) behind locomp.embed_lookup (locomp/api.py:1025-1038).  An id
@@ -336,6 +370,12 @@ int lcq_gemv_tc_plan_cluster(int M, int N, int K, int sm_count);
  * that share a tile's K, pieces per tile of the last wave}.
  */
 int lcq_gemm_tc_plan_check(int M, int N, int K, int sm_count, int* fields);
+
+/*
+ * The same check for the int8 product; aligned_rows: whether TMA can read x and w.  fields (may be NULL) receives {CTAs, tokens per
+ * tile, tiles, tiles cut along K, shared-memory bytes, CTAs per MMA, CTAs per cluster that share a tile's K, stages in the ring}.
+ */
+int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int aligned_rows, int* fields);
 
 /*
  * The same check for the decode-step kernel (only the sizes of `stack` are read): every row in the stages of one CTA, every

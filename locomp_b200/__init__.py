@@ -11,6 +11,7 @@ from .ops import (dequant_int4, dequant_int8, dequant_matvec_int4, dequant_matve
 from .decode_ops import (QuantizedWeight, add_inplace, add_inplace_kernel, argmax, embed_lookup, quantize, quantize_int4,
                          quantize_int4_ref, quantize_int8, residual_rms_norm, rms_norm, rms_norm_kernel, silu_mul,
                          silu_mul_kernel)
+from .int8_ops import Int8Linear, QuantizedTokens, int8_matmul, quantize_tokens, residual_norms, silu_mul_tokens
 from .linear import DecodeStack, QuantLinear, fuse_rows
 from .shard import PeerGather, ShardedQuantLinear, shard_rows
 from .tensor import DeviceTensor, empty, tensor, zeros
@@ -22,5 +23,6 @@ __all__ = [
     "quantized_matmul", "dequantize", "rms_norm", "residual_rms_norm", "silu_mul", "add_inplace", "embed_lookup", "argmax",
     "rms_norm_kernel", "silu_mul_kernel", "add_inplace_kernel", "quantize", "quantize_int4", "quantize_int8",
     "quantize_int4_ref", "QuantizedWeight", "ShardedQuantLinear", "PeerGather", "shard_rows", "QuantLinear", "fuse_rows", "DecodeStack",
+    "int8_matmul", "Int8Linear", "QuantizedTokens", "quantize_tokens", "silu_mul_tokens", "residual_norms",
 ]
 __version__ = "0.1.0"

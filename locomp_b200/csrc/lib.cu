@@ -14,6 +14,8 @@
 #include "glue.cuh"
 #include "quantize.cuh"
 #include "decode_step.cuh"
+#include "int8_gemm.cuh"
+#include "token_rows.cuh"
 
 namespace lcq {
 
@@ -691,6 +693,174 @@ int lcq_argmax(const void* x, void* out, int64_t rows, int n, int dtype, void* s
   if (!x || !out) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LCQ_BY_DTYPE(dtype, (glue::launch_argmax<T>(x, out, rows, n, st)))
+}
+
+// ---------------------------------------------------------------- the int8 path: products and what stands between them
+// A single row has no row stride; any multiple of 16 that covers it will do.
+static int64_t stride_of(int64_t rows, int64_t ld, int64_t n) { return rows > 1 ? ld : (n + 15) / 16 * 16; }
+
+static int check_int8_problem(int M, int N, int K) {
+  if (M < 0 || N < 0 || K <= 0) { set_error("int8 matmul: bad sizes M=%d N=%d K=%d", M, N, K); return LCQ_ERR_BAD_ARG; }
+  if (K > int8_gemm::MAX_K) { set_error("int8 matmul: K=%d is more than int32 sums hold (%d)", K, int8_gemm::MAX_K); return LCQ_ERR_UNSUPPORTED; }
+  if ((static_cast<int64_t>(M) + 15) / 16 * ((static_cast<int64_t>(N) + 127) / 128) > (1 << 30)) {
+    set_error("int8 matmul: M=%d by N=%d is more than 2^30 tiles", M, N);
+    return LCQ_ERR_UNSUPPORTED;
+  }
+  return LCQ_OK;
+}
+
+int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, void* out,
+                    int M, int N, int K, int w_scale_dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = check_int8_problem(M, N, K);
+  if (rc != LCQ_OK) return rc;
+  if (!dtype_ok(w_scale_dtype) || !dtype_ok(out_dtype)) { set_error("bad dtype code"); return LCQ_ERR_BAD_ARG; }
+  if (M == 0 || N == 0) return LCQ_OK;
+  if (!x || !x_scales || !w || !w_scales || !out) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
+  if ((M > 1 && ldx < K) || (N > 1 && ldw < K)) { set_error("int8 matmul: rows of x and w must be at least K=%d apart", K); return LCQ_ERR_BAD_ARG; }
+  DevInfo di;
+  rc = current_dev_info(di);
+  if (rc != LCQ_OK) return rc;
+  if (di.major != 10) { set_error("tensor-core kernels are built for sm_100a only; device is sm_%d%d", di.major, di.minor); return LCQ_ERR_UNSUPPORTED; }
+  ldx = stride_of(M, ldx, K);
+  ldw = stride_of(N, ldw, K);
+  const bool loader = !int8_gemm::mappable(x, ldx) || !int8_gemm::mappable(w, ldw);
+  return int8_gemm::launch_tiling(int8_gemm::choose_tiling(M, N, K, di.sm_count, loader), x, ldx, x_scales, w, ldw, w_scales, out, M, N, K,
+                                  w_scale_dtype, out_dtype, loader, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+}
+
+size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K) {
+  if (check_int8_problem(M, N, K) != LCQ_OK) return static_cast<size_t>(-1);
+  if (M == 0 || N == 0) return 0;
+  int sm = 148, dev = 0, v = 0;
+  if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0) sm = v;
+  const size_t a = int8_gemm::workspace_bytes(int8_gemm::choose_tiling(M, N, K, sm, false));
+  const size_t b = int8_gemm::workspace_bytes(int8_gemm::choose_tiling(M, N, K, sm, true));
+  return a > b ? a : b;
+}
+
+// Replays the schedule of all teams: every (tile, stage) once, contributors and slots of the cut tiles as the kernel derives them.
+int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int aligned_rows, int* fields) {
+  using namespace int8_gemm;
+  int rc = check_int8_problem(M, N, K);
+  if (rc != LCQ_OK) return rc;
+  if (M == 0 || N == 0 || sm_count <= 0) { set_error("int8 plan: nothing to plan"); return LCQ_ERR_BAD_ARG; }
+  const Tiling t = choose_tiling(M, N, K, sm_count, !aligned_rows);
+  const Params p = make_params(t, M, N, K);
+  const int smem = smem_map(p.bm, t.cg, p.depth).total;
+  if (fields) {
+    const int f[8] = {t.cg * t.teams, t.bm, t.n_tiles, t.sk_tiles, smem, t.cg, t.split, t.depth};
+    memcpy(fields, f, sizeof(f));
+  }
+  const auto wrong = [](const char* what) { set_error("int8 plan: %s", what); return LCQ_ERR_BAD_ARG; };
+  if (smem > 227 * 1024 || t.depth < 2 || t.depth > MAX_STAGES) return wrong("shared memory");
+  if (t.bm % (16 * t.cg) != 0 || t.bm > 256 || p.tmem_cols > 512 || t.bm + (t.bm + 31) / 32 * 32 > p.tmem_cols) return wrong("tensor memory");
+  if (static_cast<size_t>(t.sk_tiles) * t.cg * sizeof(int) > kWorkspaceCounterBytes) return wrong("counters");
+  if (t.split > 1 && (t.cg != 1 || t.teams != t.n_tiles * t.split || (p.bm + t.split - 1) / t.split * t.split * BN * 4 > t.depth * stage_bytes(p.bm, 1)))
+    return wrong("cluster");
+  if (t.split == 1 && t.cg * t.teams > sm_count) return wrong("more CTAs than SMs");
+  std::vector<uint8_t> seen(static_cast<size_t>(t.n_tiles) * p.nst), place(static_cast<size_t>(t.tn) * t.tm);
+  std::vector<int> contributors(t.sk_tiles, 0);
+  std::vector<int> slot_tile(static_cast<size_t>(t.teams) * 2, -1);
+  for (int team = 0; team < t.teams; ++team) {
+    int last_tile = -1;
+    for (Walk w(p, team); w.next(p);) {
+      if (w.tile < 0 || w.tile >= t.n_tiles || w.st0 < 0 || w.st1 > p.nst || w.st0 >= w.st1) return wrong("segment out of range");
+      if (w.nt < 0 || w.nt >= t.tn || w.mt < 0 || w.mt >= t.tm) return wrong("tile out of place");
+      if (w.st0 == 0) {
+        if (place[static_cast<size_t>(w.mt) * t.tn + w.nt]++) return wrong("two tiles in one place");
+      }
+      for (int st = w.st0; st < w.st1; ++st)
+        if (seen[static_cast<size_t>(w.tile) * p.nst + st]++) return wrong("a stage twice");
+      if (w.tile < p.sk_tiles) {
+        const unsigned t0 = static_cast<unsigned>(w.tile) * static_cast<unsigned>(p.nst);
+        const int p0 = share_owner(p, t0), p1 = share_owner(p, t0 + static_cast<unsigned>(p.nst) - 1u);
+        if (team < p0 || team > p1) return wrong("contributor out of range");
+        ++contributors[w.tile];
+        if (p1 != p0) {
+          const int slot = team == p0 && share_begin(p, p0) < t0;
+          int& holds = slot_tile[static_cast<size_t>(team) * 2 + slot];
+          if (holds >= 0) return wrong("a slot twice");
+          holds = w.tile;
+        }
+      }
+      if (w.tile == last_tile) return wrong("a tile twice in one team");
+      last_tile = w.tile;
+    }
+  }
+  for (uint8_t s : seen) if (s != 1) return wrong("a stage left out");
+  for (uint8_t s : place) if (s != 1) return wrong("a place left out");
+  for (int i = 0; i < t.sk_tiles; ++i) {
+    const unsigned t0 = static_cast<unsigned>(i) * static_cast<unsigned>(p.nst);
+    if (contributors[i] != share_owner(p, t0 + static_cast<unsigned>(p.nst) - 1u) - share_owner(p, t0) + 1) return wrong("contributors of a cut tile");
+  }
+  return LCQ_OK;
+}
+
+static int check_rows(const char* what, int64_t rows, int n) {
+  if (rows < 0 || n < 0) { set_error("%s: negative size", what); return LCQ_ERR_BAD_ARG; }
+  if (n > (1 << 30)) { set_error("%s: rows of %d values are not supported", what, n); return LCQ_ERR_UNSUPPORTED; }
+  return LCQ_OK;
+}
+
+int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q, int64_t ldq, void* scales, int64_t rows, int n, float eps,
+                        int dtype, void* stream) {
+  int rc = check_rows("quantize_tokens", rows, n);
+  if (rc != LCQ_OK) return rc;
+  if (rows == 0 || n == 0) return LCQ_OK;
+  if (!x || !q || !scales) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
+  if (rows > 1 && (ldx < n || ldq < n)) { set_error("quantize_tokens: rows must be at least n=%d apart", n); return LCQ_ERR_BAD_ARG; }
+  rows::Args a = {};
+  a.a = x; a.lda = stride_of(rows, ldx, n);
+  a.weight = weight;
+  a.out = q; a.ldo = stride_of(rows, ldq, n);
+  a.scales = static_cast<float*>(scales);
+  a.n_rows = rows; a.n = n; a.eps = eps;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::ROWS, true>(a, st)))
+}
+
+int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* q, int64_t ldq, void* scales, int64_t rows,
+                        int n, int dtype, void* stream) {
+  int rc = check_rows("silu_mul_tokens", rows, n);
+  if (rc != LCQ_OK) return rc;
+  if (rows == 0 || n == 0) return LCQ_OK;
+  if (!gate || !up || !q || !scales) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
+  if (rows > 1 && (ld_gate < n || ld_up < n || ldq < n)) { set_error("silu_mul_tokens: rows must be at least n=%d apart", n); return LCQ_ERR_BAD_ARG; }
+  rows::Args a = {};
+  a.a = gate; a.lda = stride_of(rows, ld_gate, n);
+  a.b = up; a.ldb = stride_of(rows, ld_up, n);
+  a.out = q; a.ldo = stride_of(rows, ldq, n);
+  a.scales = static_cast<float*>(scales);
+  a.n_rows = rows; a.n = n;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::SILU_MUL, true>(a, st)))
+}
+
+int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
+                       const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n, float eps, int dtype,
+                       void* stream) {
+  int rc = check_rows("residual_norms", rows, n);
+  if (rc != LCQ_OK) return rc;
+  if (rows == 0 || n == 0) return LCQ_OK;
+  if (!hidden || !delta || !hidden_out || (weight && !out)) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
+  if (scales && !weight) { set_error("residual_norms: int8 tokens are those of the norm, which needs a weight"); return LCQ_ERR_BAD_ARG; }
+  if (gate && (gate_rows <= 0 || rows % gate_rows != 0)) {
+    set_error("residual_norms: %lld rows are not a multiple of %lld gate rows", static_cast<long long>(rows), static_cast<long long>(gate_rows));
+    return LCQ_ERR_BAD_ARG;
+  }
+  if (weight && rows > 1 && ld_out < n) { set_error("residual_norms: rows of out must be at least n=%d apart", n); return LCQ_ERR_BAD_ARG; }
+  rows::Args a = {};
+  a.a = hidden; a.lda = n;
+  a.b = delta; a.ldb = n;
+  a.weight = weight; a.post_weight = post_weight; a.gate = gate;
+  a.rows_per_gate = gate ? rows / gate_rows : 1;
+  a.hidden_out = hidden_out;
+  a.out = weight ? out : nullptr; a.ldo = weight ? stride_of(rows, ld_out, n) : 0;
+  a.scales = static_cast<float*>(scales);
+  a.n_rows = rows; a.n = n; a.eps = eps; a.scale = scale;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (scales) { LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, true>(a, st))) }
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, false>(a, st)))
 }
 
 // ---------------------------------------------------------------- one kernel per decode step

@@ -21,6 +21,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -41,6 +42,11 @@ struct Api {
   decltype(&lcq_embed_lookup) embed_lookup;
   decltype(&lcq_argmax) argmax;
   decltype(&lcq_matmul_workspace_bytes) workspace_bytes;
+  decltype(&lcq_int8_matmul) int8_matmul;
+  decltype(&lcq_int8_matmul_workspace_bytes) int8_workspace_bytes;
+  decltype(&lcq_quantize_tokens) quantize_tokens;
+  decltype(&lcq_silu_mul_tokens) silu_mul_tokens;
+  decltype(&lcq_residual_norms) residual_norms;
 } api;
 PyObject* raise_status = nullptr;      // callable(status): raises the exception of a negative status
 PyObject* make_workspace = nullptr;    // callable(nbytes, device, stream): allocates (or grows) and reports it through set_workspace
@@ -306,6 +312,213 @@ PyObject* add_inplace(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return finish(unlocked([&] { return api.add_inplace(a->data_ptr(), b->data_ptr(), a->numel(), code, stream); }), args[0]);
 }
 
+// A CUDA tensor whose rows (its last dimension) are contiguous and equally far apart, `ld` elements; or nullptr.
+const at::Tensor* row_tensor(PyObject* o, int64_t& ld) {
+  if (!THPVariable_CheckExact(o)) return nullptr;
+  const at::Tensor& t = THPVariable_Unpack(o);
+  if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() < 1 || t.numel() == 0) return nullptr;
+  const int64_t n = t.size(-1);
+  ld = n;
+  if (t.is_contiguous()) return &t;
+  if (n != 1 && t.stride(-1) != 1) return nullptr;
+  int64_t span = 0;                      // of the dimensions seen so far
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (span == 0) ld = t.stride(d);
+    else if (t.stride(d) != span) return nullptr;
+    span = t.stride(d) * t.size(d);
+  }
+  return ld >= n ? &t : nullptr;
+}
+// The int8 rows and scales that a call writes: new ones, or the tensors of the pair `given`.
+struct Tokens {
+  at::Tensor q, scales;
+  int64_t ld = 0;
+  bool made = false;
+  bool set(PyObject* given, const at::Tensor& like) {
+    const int64_t n = like.size(-1), rows = like.numel() / n;
+    if (given == Py_None) {
+      c10::SmallVector<int64_t, 6> shape(like.sizes().begin(), like.sizes().end());
+      shape.back() = ld = (n + 15) / 16 * 16;            // rows on 16 bytes
+      q = empty(shape, at::kChar, like);
+      if (ld != n) q = q.slice(-1, 0, n);
+      scales = empty(like.sizes().slice(0, like.dim() - 1), at::kFloat, like);
+      return made = true;
+    }
+    if (!PyTuple_Check(given) || PyTuple_GET_SIZE(given) != 2) return false;
+    const at::Tensor *a = row_tensor(PyTuple_GET_ITEM(given, 0), ld), *b = cuda_tensor(PyTuple_GET_ITEM(given, 1));
+    if (!a || !b || a->scalar_type() != at::kChar || a->numel() != like.numel() || a->size(-1) != n || a->device() != like.device() ||
+        b->scalar_type() != at::kFloat || b->numel() != rows || b->device() != like.device())
+      return false;
+    q = *a;
+    scales = *b;
+    return true;
+  }
+  PyObject* finish(int status) {
+    if (status < 0) return fail(status);
+    if (!made) Py_RETURN_NONE;
+    PyObject* pair = PyTuple_New(2);
+    if (!pair) return nullptr;
+    PyTuple_SET_ITEM(pair, 0, THPVariable_Wrap(std::move(q)));
+    PyTuple_SET_ITEM(pair, 1, THPVariable_Wrap(std::move(scales)));
+    return pair;
+  }
+};
+constexpr int64_t MOST_PER_ROW = 1 << 30;
+
+// quantize_tokens(x, weight | None, eps, (q, scales) | None) -> (q, scales), or None where they were given
+PyObject* quantize_tokens(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 4) return not_implemented();
+  int64_t ld;
+  const at::Tensor *x = row_tensor(args[0], ld), *w = nullptr;
+  if (!x || !PyFloat_Check(args[2]) || float_code(x->scalar_type()) == NOT_FLOAT) return not_implemented();
+  const int64_t n = x->size(-1);
+  if (args[1] != Py_None && (!(w = cuda_tensor(args[1])) || shared_code(*x, *w) == NOT_FLOAT || w->numel() != n)) return not_implemented();
+  if (n > MOST_PER_ROW) return not_implemented();
+  const c10::cuda::OptionalCUDAGuard guard(x->device());
+  Tokens t;
+  if (!t.set(args[3], *x)) return not_implemented();
+  void* stream = current_stream(x->device().index());
+  const float eps = static_cast<float>(PyFloat_AS_DOUBLE(args[2]));
+  return t.finish(unlocked([&] {
+    return api.quantize_tokens(x->data_ptr(), ld, w ? w->data_ptr() : nullptr, t.q.data_ptr(), t.ld, t.scales.data_ptr(), x->numel() / n,
+                               static_cast<int>(n), eps, float_code(x->scalar_type()), stream);
+  }));
+}
+
+// silu_mul_tokens(gate, up, (q, scales) | None) -> (q, scales), or None where they were given
+PyObject* silu_mul_tokens(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 3) return not_implemented();
+  int64_t ldg, ldu;
+  const at::Tensor *g = row_tensor(args[0], ldg), *u = row_tensor(args[1], ldu);
+  if (!g || !u || g->sizes() != u->sizes() || g->size(-1) > MOST_PER_ROW) return not_implemented();
+  const int code = shared_code(*g, *u);
+  if (code == NOT_FLOAT) return not_implemented();
+  const int64_t n = g->size(-1);
+  const c10::cuda::OptionalCUDAGuard guard(g->device());
+  Tokens t;
+  if (!t.set(args[2], *g)) return not_implemented();
+  void* stream = current_stream(g->device().index());
+  return t.finish(unlocked([&] {
+    return api.silu_mul_tokens(g->data_ptr(), ldg, u->data_ptr(), ldu, t.q.data_ptr(), t.ld, t.scales.data_ptr(), g->numel() / n,
+                               static_cast<int>(n), code, stream);
+  }));
+}
+
+// residual_norms(hidden, delta, weight | None, eps, post_weight | None, gate | None, scale, hidden_out | None, out | (q, scales) | None, quantized)
+// -> the norm, (q, scales) or the new hidden; None where `out` was given
+PyObject* residual_norms(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 10) return not_implemented();
+  const at::Tensor *h = cuda_tensor(args[0]), *d = cuda_tensor(args[1]);
+  if (!h || !d || h->dim() < 1 || h->numel() == 0 || !PyFloat_Check(args[3]) || !PyFloat_Check(args[6]) || !PyBool_Check(args[9]))
+    return not_implemented();
+  const int64_t n = h->size(-1), rows = h->numel() / n;
+  const int code = shared_code(*h, *d);
+  if (code == NOT_FLOAT || d->dim() < 1 || d->numel() != h->numel() || d->size(-1) != n || n > MOST_PER_ROW) return not_implemented();
+  const at::Tensor* more[3] = {nullptr, nullptr, nullptr};        // weight, post_weight, gate
+  const int where[3] = {2, 4, 5};
+  for (int i = 0; i < 3; ++i) {
+    if (args[where[i]] == Py_None) continue;
+    more[i] = cuda_tensor(args[where[i]]);
+    if (!more[i] || shared_code(*h, *more[i]) == NOT_FLOAT || (i < 2 && more[i]->numel() != n)) return not_implemented();
+  }
+  const bool quantized = args[9] == Py_True;
+  if (!more[0] && (quantized || args[8] != Py_None)) return not_implemented();
+  int64_t gate_rows = 0;
+  if (more[2]) {
+    gate_rows = more[2]->numel() / n;
+    if (more[2]->dim() < 1 || more[2]->size(-1) != n || gate_rows == 0 || rows % gate_rows != 0) return not_implemented();
+  }
+  const at::Tensor* ho = h;
+  if (args[7] != Py_None && (!(ho = cuda_tensor(args[7])) || ho->numel() != h->numel() || shared_code(*h, *ho) == NOT_FLOAT))
+    return not_implemented();
+  const c10::cuda::OptionalCUDAGuard guard(h->device());
+  Tokens t;
+  at::Tensor made;
+  const at::Tensor* out = nullptr;
+  if (quantized) {
+    if (!t.set(args[8], *h)) return not_implemented();
+  } else if (more[0] && !(out = result(args[8], *h, made))) {
+    return not_implemented();
+  }
+  void* stream = current_stream(h->device().index());
+  const float eps = static_cast<float>(PyFloat_AS_DOUBLE(args[3])), scale = static_cast<float>(PyFloat_AS_DOUBLE(args[6]));
+  const auto ptr = [](const at::Tensor* a) { return a ? a->data_ptr() : nullptr; };
+  const int rc = unlocked([&] {
+    return api.residual_norms(h->data_ptr(), d->data_ptr(), ptr(more[1]), ptr(more[2]), gate_rows, scale, ptr(more[0]), ho->data_ptr(),
+                              quantized ? t.q.data_ptr() : ptr(out), quantized ? t.ld : n, quantized ? t.scales.data_ptr() : nullptr, rows,
+                              static_cast<int>(n), eps, code, stream);
+  });
+  if (quantized) return t.finish(rc);
+  if (!more[0]) return finish(rc, args[7] == Py_None ? args[0] : args[7]);
+  return args[8] == Py_None ? finish(rc, std::move(made)) : finish(rc, Py_None);
+}
+
+// int8_matmul(x, x_scales, w, w_scales, out | None, out dtype code | -1, workspace | None)
+PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 7) return not_implemented();
+  int64_t ldx, ldw;
+  const at::Tensor *x = row_tensor(args[0], ldx), *xs = cuda_tensor(args[1]), *w = row_tensor(args[2], ldw), *ws = cuda_tensor(args[3]);
+  long long wanted;
+  if (!x || !xs || !w || !ws || !as_int(args[5], wanted) || wanted < -1 || wanted > LCQ_BF16) return not_implemented();
+  if (x->scalar_type() != at::kChar || w->scalar_type() != at::kChar || xs->scalar_type() != at::kFloat) return not_implemented();
+  const bool row = x->dim() == 1;
+  if ((!row && x->dim() != 2) || w->dim() != 2 || w->device() != x->device() || xs->device() != x->device() || ws->device() != x->device())
+    return not_implemented();
+  const int64_t M = row ? 1 : x->size(0), K = x->size(-1), N = w->size(0);
+  constexpr int64_t most = 2000000000;
+  const int sk = float_code(ws->scalar_type());
+  if (w->size(1) != K || xs->numel() != M || ws->numel() != N || sk == NOT_FLOAT || M > most || N > most || K > most) return not_implemented();
+  at::Tensor made;
+  const at::Tensor* out = &made;
+  int ok = wanted < 0 ? LCQ_F16 : static_cast<int>(wanted);
+  const c10::cuda::OptionalCUDAGuard guard(x->device());
+  if (args[4] == Py_None) {
+    made = row ? empty({N}, float_type(ok), *x) : empty({M, N}, float_type(ok), *x);
+  } else {
+    out = cuda_tensor(args[4]);
+    if (!out || out->device() != x->device() || out->numel() != M * N) return not_implemented();
+    const int given = float_code(out->scalar_type());
+    if (given == NOT_FLOAT || (wanted >= 0 && given != ok)) return not_implemented();
+    ok = given;
+  }
+  const int dev = x->device().index();
+  void* stream = current_stream(dev);
+  const void *xp = x->data_ptr(), *wp = w->data_ptr(), *xsp = xs->data_ptr(), *wsp = ws->data_ptr();
+  void* op = out->data_ptr();
+  const auto call = [&](void* scratch, size_t bytes) {     // without the GIL
+    return api.int8_matmul(xp, ldx, xsp, wp, ldw, wsp, op, static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), sk, ok, scratch, bytes, stream);
+  };
+  int rc;
+  if (args[6] != Py_None) {
+    const at::Tensor* given = cuda_tensor(args[6]);
+    if (!given || given->device() != x->device()) return not_implemented();
+    void* ptr = given->data_ptr();
+    const size_t bytes = given->nbytes();
+    rc = unlocked([&] { return call(ptr, bytes); });
+    if (rc == LCQ_ERR_WORKSPACE) return not_implemented();
+  } else if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
+    rc = unlocked([&] { return call(nullptr, 0); });
+    if (rc == LCQ_ERR_WORKSPACE) return not_implemented();   // (the general path gives the graph scratch of its own)
+  } else {
+    Scratch& scratch = scratches[{dev, reinterpret_cast<uintptr_t>(stream)}];
+    NoGil released;
+    const std::lock_guard<std::recursive_mutex> held(scratch.lock);
+    rc = call(scratch.ptr, scratch.bytes);
+    if (rc == LCQ_ERR_WORKSPACE) {
+      released.end();
+      const size_t need = api.int8_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+      PyObject* r = PyObject_CallFunction(make_workspace, "niK", static_cast<Py_ssize_t>(need), dev,
+                                          static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)));
+      if (!r) return nullptr;
+      Py_DECREF(r);
+      released.again();
+      rc = call(scratch.ptr, scratch.bytes);
+    }
+  }
+  return args[4] == Py_None ? finish(rc, std::move(made)) : finish(rc, args[4]);
+}
+
 // embed_lookup(token_ids, table, out, seq_len, dim)
 PyObject* embed_lookup(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (n_args != 5) return not_implemented();
@@ -411,6 +624,11 @@ PyObject* bind(PyObject*, PyObject* args) {
   find(api.embed_lookup, "lcq_embed_lookup");
   find(api.argmax, "lcq_argmax");
   find(api.workspace_bytes, "lcq_matmul_workspace_bytes");
+  find(api.int8_matmul, "lcq_int8_matmul");
+  find(api.int8_workspace_bytes, "lcq_int8_matmul_workspace_bytes");
+  find(api.quantize_tokens, "lcq_quantize_tokens");
+  find(api.silu_mul_tokens, "lcq_silu_mul_tokens");
+  find(api.residual_norms, "lcq_residual_norms");
   if (!all) return PyErr_Format(PyExc_ImportError, "%s lacks an entry point", path);
   Py_INCREF(raise_fn);
   Py_INCREF(workspace_fn);
@@ -472,6 +690,7 @@ PyObject* guarded(PyObject* self, PyObject* const* args, Py_ssize_t n) {
 PyMethodDef methods[] = {
     LCQ_METHOD(matmul), LCQ_METHOD(dequantize), LCQ_METHOD(quantize), LCQ_METHOD(rms_norm), LCQ_METHOD(residual_rms_norm),
     LCQ_METHOD(silu_mul), LCQ_METHOD(add_inplace), LCQ_METHOD(embed_lookup), LCQ_METHOD(argmax), LCQ_METHOD(set_workspace),
+    LCQ_METHOD(quantize_tokens), LCQ_METHOD(silu_mul_tokens), LCQ_METHOD(residual_norms), LCQ_METHOD(int8_matmul),
     LCQ_METHOD(lock_workspace), LCQ_METHOD(unlock_workspace),
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

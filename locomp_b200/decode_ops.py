@@ -286,6 +286,13 @@ class QuantizedWeight:
         from .linear import QuantLinear
         return QuantLinear(self.w, self.scales, self.group_size, self.bits)
 
+    def int8_linear(self):
+        """The layer that multiplies int8 tokens (Int8Linear)."""
+        from .int8_ops import Int8Linear
+        if self.bits != 8 or self.group_size != self.shape[1]:
+            raise ValueError("int8 products take int8 weights with one scale per output channel: quantize(weights, K, bits=8)")
+        return Int8Linear(self.w, self.scales)
+
 
 def quantize(weights, group_size: int = 32, *, bits: int = 4, style: str = "ex38", scale_dtype: Optional[str] = None,
              stream=None) -> QuantizedWeight:
