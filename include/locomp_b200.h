@@ -179,8 +179,10 @@ int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
  *   x int8 [M, K] with rows ldx bytes apart, x_scales float32 [M]; w int8 [N, K] with rows ldw bytes apart, w_scales [N] of
  *   w_scale_dtype (lcq_quantize_int8 with group_size = K makes both); out [M, N] of out_dtype, contiguous.  The sum is an exact
  *   int32 (K <= 131071, else LCQ_ERR_UNSUPPORTED), the scales are applied in float32, the result is rounded once.  Rows on 16 bytes
- *   (x, w, ldx, ldw multiples of 16) are read by TMA; any other are fetched by slower loads.
- *   workspace: as for lcq_matmul_int4, of lcq_int8_matmul_workspace_bytes() bytes; the same buffer may serve both.  Nothing is read
+ *   (x, w, ldx, ldw multiples of 16; ld does not matter to a single row) are read where they are, any other are first copied into the
+ *   workspace: x whole, w at most 48 MiB at a time.
+ *   workspace: of lcq_int8_matmul_workspace_bytes() bytes, 256-byte aligned, for those copies (none: NULL); it need not be cleared, and a buffer of
+ *   lcq_matmul_int4 may serve.  Nothing is read
  *   before the kernel ahead on the stream has completed: unlike lcq_matmul_int4, weights may be written by it.
  *
  * lcq_quantize_tokens: q[r, :] = rint(v / s), scales[r] = s = max|v| / 127 with v = x[r, :] or, where `weight` is given,
@@ -196,7 +198,7 @@ int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
  */
 int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, void* out,
                     int M, int N, int K, int w_scale_dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
-size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K);
+size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K, int x_on_16, int w_on_16);   /* whether rows of x, of w start on 16 bytes */
 int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q, int64_t ldq, void* scales, int64_t rows, int n,
                         float eps, int dtype, void* stream);
 int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* q, int64_t ldq, void* scales,
@@ -372,10 +374,11 @@ int lcq_gemv_tc_plan_cluster(int M, int N, int K, int sm_count);
 int lcq_gemm_tc_plan_check(int M, int N, int K, int sm_count, int* fields);
 
 /*
- * The same check for the int8 product; aligned_rows: whether TMA can read x and w.  fields (may be NULL) receives {CTAs, tokens per
- * tile, tiles, tiles cut along K, shared-memory bytes, CTAs per MMA, CTAs per cluster that share a tile's K, stages in the ring}.
+ * The same check for the int8 product; w_on_16: whether rows of w start on 16 bytes.  fields (may be NULL) receives {CTAs, tokens per
+ * tile, tiles, tiles in pieces of fewer tokens, shared-memory bytes, CTAs per MMA, CTAs per cluster that share a tile's K, stages in the ring,
+ * weight rows of a product (N, or fewer where they are copied in pieces)}.
  */
-int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int aligned_rows, int* fields);
+int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int w_on_16, int* fields);
 
 /*
  * The same check for the decode-step kernel (only the sizes of `stack` are read): every row in the stages of one CTA, every

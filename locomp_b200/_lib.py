@@ -48,7 +48,7 @@ SIGNATURES = {
     "lcq_add_inplace": (_c.c_int, [_c.c_void_p] * 2 + [_c.c_int64, _c.c_int, _c.c_void_p]),
     "lcq_int8_matmul": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p] +
                         [_c.c_int] * 5 + [_c.c_void_p, _c.c_size_t, _c.c_void_p]),
-    "lcq_int8_matmul_workspace_bytes": (_c.c_size_t, [_c.c_int] * 3),
+    "lcq_int8_matmul_workspace_bytes": (_c.c_size_t, [_c.c_int] * 5),
     "lcq_int8_matmul_plan_check": (_c.c_int, [_c.c_int] * 5 + [_c.POINTER(_c.c_int)]),
     "lcq_quantize_tokens": (_c.c_int, [_c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_void_p, _c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int,
                                        _c.c_float, _c.c_int, _c.c_void_p]),

@@ -150,7 +150,7 @@ __device__ __forceinline__ void opaque_zero4(float (&z)[4]) {
 // ------------------------------------------------------------------ tensor-map encoding (host)
 // Encodes a 2-D row-major tensor map through the driver entry point obtained at run time,
 // so the library has no link-time dependency on libcuda.
-int encode_tmap_2d(void* out_map /*CUtensorMap, 128 B*/, int dtype_code /*0=u8,1=f16,2=bf16*/,
+int encode_tmap_2d(void* out_map /*CUtensorMap, 128 B*/, int dtype_code /*0=u8,1=f16,2=bf16,3=f32*/,
                    const void* base, uint64_t inner, uint64_t outer, uint64_t row_stride_bytes,
                    uint32_t box_inner, uint32_t box_outer, int swizzle_code /*0 none,1=32B,2=64B,3=128B*/);
 

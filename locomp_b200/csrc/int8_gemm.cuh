@@ -13,15 +13,16 @@
 // of stages does nothing but stream weights.
 // A lane of the accumulator is a channel: its scale is one register, and a warp stores 32 consecutive channels of a token.
 //
-// Split of the work: whole tiles in turn while they fill all teams; the rest is cut along K into equal shares, whose
-// int32 partials meet through scratch (the last contributor adds them up; nobody waits for another CTA), or, where there
-// are few tiles, a cluster of CTAs shares the K of each tile and adds up over distributed shared memory.
+// Split of the work: whole tiles in turn while they fill all teams, the rest in pieces of fewer tokens; or, where there are few tiles, a
+// cluster of CTAs shares the K of each tile and adds up over distributed shared memory.  (Cutting the last tiles along K between CTAs that meet
+// through scratch was faster for 4 problems of 75, by 3 %, and made every call need scratch.)
 //
 // The weights' first stages are fetched into L2 while the kernel before this one still runs.  L2 is where all SMs' stores
 // meet, so this is right whoever writes the weights; everything is read after that kernel has completed.
 //
-// LOADER: operands whose rows do not start on 16 bytes (K % 16 != 0 in contiguous storage, or an odd offset) have no
-// tensor map.  Eight warps fetch them in words, shift and store them where TMA would have put them.
+// Operands whose rows do not start on 16 bytes (K % 16 != 0 in contiguous storage, or an odd offset) have no tensor map.  They are first copied
+// into rows that do, the weights 48 MiB at a time, so that the copy is multiplied out of L2.  (Loader warps that shifted the bytes on their way into
+// the ring took two to four times as long: 333 x 4104 -> 5003 93 us, 1 x 577 -> 49152 28.6 us.)
 //
 // Every mbarrier wait is bounded; on expiry the kernel records a status code and unwinds.
 #pragma once
@@ -31,11 +32,9 @@ namespace lcq {
 namespace int8_gemm {
 
 using gemm_tc::Ring;
-using gemm_tc::all_epilogue_warps;
 using gemm_tc::arrive_leader;
 using gemm_tc::cluster_barrier;
 using gemm_tc::leader_addr;
-using gemm_tc::load_acquire;
 using gemm_tc::peer_addr;
 using gemm_tc::store_remote;
 using gemm_tc::tc_fence_after;
@@ -43,100 +42,114 @@ using gemm_tc::tc_fence_before;
 using gemm_tc::tma_load_2d_pair;
 using gemm_tc::tmem_alloc;
 using gemm_tc::tmem_dealloc;
+using gemm_tc::tmem_ld16;
 using gemm_tc::tmem_ld32;
 using gemm_tc::tmem_wait_ld;
 using gemm_tc::umma_commit;
 using gemm_tc::wait_bar;
 using gemm_tc::warp_wait;
-using gemm_tc::BAR_EPI;
 
 constexpr int BN = 128;                      // weight rows per CTA
 constexpr int BK = 128;                      // k per stage: one swizzled row of 128 bytes, four MMAs
 constexpr int W_STAGE = BN * BK;
 constexpr int MAX_STAGES = 12;
-constexpr int WARP_TMA = 4, WARP_MMA = 5, N_LOADERS = 8;     // warps 0 .. 3: epilogue
+// Warps 0 .. 7: two epilogue groups of four, which take the chunks of a tile's columns in turn (with one group, and a warp a scheduler, the
+// dependent instructions of a chunk showed: 128 x 128 tiles of 1024 k took 4.0 us each).
+constexpr int N_EPI = 8, WARP_TMA = 8, WARP_MMA = 9, NTHREADS = (WARP_MMA + 1) * 32;
+constexpr int BAR_ALL = 1, BAR_GROUP = 2;    // named barriers: both groups; group g: BAR_GROUP + g
 constexpr int MAX_K = 131071;
-constexpr int MAX_SPLIT = 8;
+constexpr int MAX_SPLIT = 8;                 // CTAs of a cluster that share a tile's K
 
-__host__ __device__ constexpr int threads(bool loader) { return (6 + (loader ? N_LOADERS : 0)) * 32; }
+// Division of 0 <= n < 2^31 by a divisor of the host's choosing: the walk's divisions by Params took 2000 clocks a tile.
+struct Divisor {
+  uint32_t mul;
+  int shift;
+  __host__ __device__ int divide(int n) const { return static_cast<int>((static_cast<uint64_t>(static_cast<uint32_t>(n)) * mul) >> shift); }
+};
+inline Divisor make_divisor(int d) {           // mul = ceil(2^(31 + l) / d), l = ceil(log2 d): exact for n < 2^31
+  int l = 0;
+  while ((1ll << l) < d) ++l;
+  const uint64_t two = 1ull << (31 + l);
+  return {static_cast<uint32_t>((two + static_cast<uint64_t>(d) - 1) / static_cast<uint64_t>(d)), 31 + l};
+}
 
 struct Params {
-  void* out;                 // [M, N]
+  void* out;                 // [M, N], rows ldo apart
   const float* x_scales;     // [M]
   const void* w_scales;      // [N]
-  const uint8_t *x, *w;      // LOADER
-  long long ldx, ldw;        // LOADER: bytes between rows
-  int* partials;             // [2 * teams * CG][bm][BN]
-  int* counters;             // [sk_tiles * CG], zero on entry, zero on exit
+  long long ldo;
   int M, N, K, w_scale_dtype;
   int bm;                    // tokens per tile (MMA N): a multiple of 16 CG, at most 256
+  int piece_bm;              // bm / tail
   int tn, tm, n_tiles;
   int group;                 // token tiles that are walked together
   int nst;                   // 128-k stages per tile
   int teams;                 // CTAs (CG = 1) or pairs (CG = 2) launched
-  int sk_tiles;              // tiles 0 .. sk_tiles - 1 are cut along K, the others go whole to team (tile - sk_tiles) % teams
+  int full, tail;            // tiles full .. are cut into `tail` pieces of bm / tail tokens (a last wave that would be mostly empty)
   int split;                 // > 1: a cluster of `split` CTAs per tile, each with its share of K
   int depth;                 // stages in the ring
   int tmem_cols;
+  int vec;                   // whether rows of out start on 16 bytes
+  Divisor by_group_tiles, by_group, by_last_group, by_tail;     // (tn * group tiles a group; token tiles in a group and in the last one)
 };
 
-__host__ __device__ inline unsigned share_begin(const Params& p, int team) {
-  const unsigned long long units = static_cast<unsigned long long>(p.sk_tiles) * static_cast<unsigned>(p.nst);
-  return static_cast<unsigned>(units * static_cast<unsigned>(team) / static_cast<unsigned>(p.teams));
-}
-__host__ __device__ inline int share_owner(const Params& p, unsigned unit) {
-  const unsigned long long units = static_cast<unsigned long long>(p.sk_tiles) * static_cast<unsigned>(p.nst);
-  return static_cast<int>((static_cast<unsigned long long>(unit + 1u) * static_cast<unsigned>(p.teams) - 1u) / units);
-}
-
-// The segments of one team: (tile, stages st0 .. st1 - 1).  Every role walks them in the same order.
+// The segments of one team: (tile or piece of one, stages st0 .. st1 - 1).  Every role walks them in the same order.
 struct Walk {
-  unsigned u, u1;            // what is left of the team's share of the cut tiles
-  int next_tile;
+  int item, step;            // tiles, then pieces; how far apart a team's are
   int tile, st0, st1;
   int mt, nt;                // the tile's place
+  int m0, bm;                // first token and their number
   __host__ __device__ Walk(const Params& p, int team) {
     if (p.split > 1) {
-      const int t = team / p.split, r = team - t * p.split;
-      u = static_cast<unsigned>(t * p.nst + p.nst * r / p.split);
-      u1 = static_cast<unsigned>(t * p.nst + p.nst * (r + 1) / p.split);
-      next_tile = p.n_tiles;
+      item = team / p.split;
+      const int r = team - item * p.split;
+      st0 = p.nst * r / p.split;
+      st1 = p.nst * (r + 1) / p.split;
+      step = p.n_tiles;
     } else {
-      u = share_begin(p, team);
-      u1 = share_begin(p, team + 1);
-      next_tile = p.sk_tiles + team;
+      item = team;
+      st0 = 0;
+      st1 = p.nst;
+      step = p.teams;
     }
   }
   __host__ __device__ bool next(const Params& p) {
-    if (u < u1) {
-      tile = static_cast<int>(u / static_cast<unsigned>(p.nst));
-      st0 = static_cast<int>(u - static_cast<unsigned>(tile) * static_cast<unsigned>(p.nst));
-      const unsigned left = u1 - u, in_tile = static_cast<unsigned>(p.nst - st0);
-      const unsigned take = left < in_tile ? left : in_tile;
-      st1 = st0 + static_cast<int>(take);
-      u += take;
-    } else {
-      tile = next_tile;
+    for (;;) {
+      tile = item;
+      int piece = 0;
+      bm = p.bm;
+      if (item >= p.full) {
+        const int i = item - p.full, of = p.by_tail.divide(i);
+        tile = p.full + of;
+        piece = i - of * p.tail;
+        bm = p.piece_bm;
+      }
       if (tile >= p.n_tiles) return false;
-      next_tile += p.teams;
-      st0 = 0;
-      st1 = p.nst;
+      item += step;
+      // `group` token tiles at a time against all channels, tokens first: what runs at the same time shares its operands in L2
+      const int g = p.by_group_tiles.divide(tile), in = tile - g * p.group * p.tn;
+      const bool last = p.tm - g * p.group < p.group;
+      const int rows = last ? p.tm - g * p.group : p.group;
+      nt = last ? p.by_last_group.divide(in) : p.by_group.divide(in);
+      mt = g * p.group + in - nt * rows;
+      m0 = mt * p.bm + piece * bm;
+      if (m0 < p.M) return true;               // (a piece past the last token is no work)
     }
-    // `group` token tiles at a time against all channels, tokens first: what runs at the same time shares its operands in L2
-    const int per_group = p.group * p.tn, g = tile / per_group, in = tile - g * per_group;
-    const int rows = p.tm - g * p.group < p.group ? p.tm - g * p.group : p.group;
-    nt = in / rows;
-    mt = g * p.group + in - nt * rows;
-    return true;
   }
 };
 
-enum { FLAG_ABORT, FLAG_SHARED, ISSUED_0, ISSUED_1, N_FLAGS };
-struct Smem { int bars, tmem_slot, flags, total; };         // offsets from the 1024-byte aligned base; the ring comes first
+enum { FLAG_ABORT, ISSUED_0, ISSUED_1, N_FLAGS };
+struct Smem { int out, xs, bars, tmem_slot, flags, total; };   // offsets from the 1024-byte aligned base; the ring comes first
 __host__ __device__ inline int stage_bytes(int bm, int cg) { return W_STAGE + (bm / cg) * BK; }
+// Tiles of 16 tokens are stored from registers, higher ones through shared memory (two buffers of 8 KB for each group).
+__host__ __device__ inline bool staged(int bm) { return bm > 16; }
+constexpr int OUT_BUFFER = 8192;
+constexpr int OUT_BOX = 16;                  // tokens of a copy out of it: tiles are multiples of 16, so none reaches into the next tile
 __host__ __device__ inline Smem smem_map(int bm, int cg, int depth) {
   Smem s;
-  s.bars = depth * stage_bytes(bm, cg);
+  s.out = depth * stage_bytes(bm, cg);
+  s.xs = s.out + (staged(bm) ? 4 * OUT_BUFFER : 0);         // scales of a tile's tokens; two tiles in turn
+  s.bars = s.xs + (staged(bm) ? 2 * 256 * 4 : 0);
   s.tmem_slot = s.bars + (2 * MAX_STAGES + 5) * 8;          // full, empty [MAX_STAGES]; full_d, empty_d [2]; drained
   s.flags = s.tmem_slot + 8;
   s.total = s.flags + 4 * N_FLAGS;
@@ -177,48 +190,12 @@ __device__ __forceinline__ float load_scale(const void* s, long long i, int dtyp
                             : __bfloat162float(static_cast<const __nv_bfloat16*>(s)[i]);
 }
 
-// The bytes p .. p + 15 of which the first `valid` exist; the others read as zero.  Only words that hold a byte that exists are read.
-__device__ __forceinline__ uint4 load_unaligned16(const uint8_t* p, int valid) {
-  if (valid >= 16 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) return *reinterpret_cast<const uint4*>(p);
-  const int off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 3);
-  const uint32_t* a = reinterpret_cast<const uint32_t*>(p - off);
-  uint32_t v[5];
-#pragma unroll
-  for (int j = 0; j < 5; ++j) v[j] = 4 * j < off + valid ? a[j] : 0u;
-  uint32_t r[4];
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const uint32_t word = __funnelshift_r(v[j], v[j + 1], off * 8);
-    const int left = valid - 4 * j;
-    r[j] = left >= 4 ? word : left <= 0 ? 0u : word & ((1u << (8 * left)) - 1u);
-  }
-  return make_uint4(r[0], r[1], r[2], r[3]);
-}
-// Up to `rows` rows of a stage (128 k from k0 on) into shared memory, in 128-byte swizzled rows, by 32 * N_LOADERS threads.
-__device__ __forceinline__ void load_rows(uint8_t* dst, const uint8_t* src, long long ld, int row0, int rows, int rows_left, int k0, int K, int t) {
-  constexpr int T = N_LOADERS * 32;
-  for (int i0 = t; i0 < rows * 8; i0 += 4 * T) {
-    uint4 v[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * T, r = i >> 3, k = k0 + (i & 7) * 16;
-      const bool there = i < rows * 8 && r < rows_left && k < K;
-      v[j] = there ? load_unaligned16(src + (static_cast<long long>(row0) + r) * ld + k, K - k) : make_uint4(0u, 0u, 0u, 0u);
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int i = i0 + j * T, r = i >> 3;
-      if (i < rows * 8) *reinterpret_cast<uint4*>(dst + r * 128 + (((i & 7) ^ (r & 7)) << 4)) = v[j];
-    }
-  }
-}
-
 // After a wait ran out in the CTA or its partner: waits for what they still have under way (the MMAs, and the copies into the last
 // stages, which nobody waits for any more).  A CTA of a pair may have loaded its part of a stage whose other part was
 // never issued: the barrier is then given the missing part, or armed for the one that comes.  All threads; in a pair between two
 // cluster barriers.
-template <int CG, bool LOADER>
-__device__ __noinline__ void drain(const Params& p, uint8_t* smem, uint32_t crank) {
+template <int CG>
+__device__ __noinline__ void drain(const Params& p, uint8_t* smem, int team, uint32_t crank) {
   const Smem L = smem_map(p.bm, CG, p.depth);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
   uint64_t* drained = full + 2 * MAX_STAGES + 4;
@@ -228,36 +205,122 @@ __device__ __noinline__ void drain(const Params& p, uint8_t* smem, uint32_t cran
     if (crank == 0) umma_commit<CG>(drained);
     __syncwarp();
     mbar_wait_landed(drained, 0);
-  } else if (!LOADER && warp == WARP_TMA && lane == 0 && crank == 0) {
+  } else if (warp == WARP_TMA && lane == 0 && crank == 0) {
     const int mine = flags[ISSUED_0], other = CG == 2 ? flags[ISSUED_1] : mine, n = mine > other ? mine : other;
-    const int bytes = stage_bytes(p.bm, CG);
-    for (int i = n > p.depth ? n - p.depth : 0; i < n; ++i) {
-      uint64_t* bar = full + i % p.depth;
-      if (i >= mine) mbar_expect_tx(bar, bytes);
-      else if (i >= other) asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
-      mbar_wait_landed(bar, (i / p.depth) & 1);
+    int i = 0;
+    for (Walk w(p, team); i < n && w.next(p);) {
+      for (int st = w.st0; st < w.st1 && i < n; ++st, ++i) {
+        if (i < n - p.depth) continue;
+        const int bytes = stage_bytes(w.bm, CG);
+        uint64_t* bar = full + i % p.depth;
+        if (i >= mine) mbar_expect_tx(bar, bytes);
+        else if (i >= other) asm volatile("mbarrier.complete_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes) : "memory");
+        mbar_wait_landed(bar, (i / p.depth) & 1);
+      }
     }
   }
   __syncthreads();
 }
 
-// 32 columns (tokens) of a tile from column c0 on: this lane's channel of each.
-template <typename OT>
-__device__ __forceinline__ void store_columns(const uint32_t (&v)[32], OT* out, long long N, bool there, int c0, int rows, const float* x_scales, float ws, int lane) {
-  const float xs = c0 + lane < rows ? x_scales[c0 + lane] : 0.0f;
-  OT* o = out + static_cast<long long>(c0) * N;
+// A chunk of columns (tokens) of a tile, as the epilogue takes them: 8 KB of output.
+template <typename OT> __host__ __device__ constexpr int chunk_columns() { return sizeof(OT) == 2 ? 32 : 16; }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[32]) { tmem_ld32(taddr, v); }
+__device__ __forceinline__ void tmem_load(uint32_t taddr, uint32_t (&v)[16]) { tmem_ld16(taddr, v); }
+__device__ __forceinline__ float scaled(uint32_t sum, float xs, float ws) { return static_cast<float>(static_cast<int>(sum)) * xs * ws; }
+
+// Stores a chunk from registers: 32 channels of a token at a time.
+template <typename OT, int C>
+__device__ __forceinline__ void store_direct(const uint32_t (&v)[C], OT* out, long long ldo, bool there, int columns, const float* x_scales, float ws, int lane) {
+  const float xs = lane < columns ? x_scales[lane] : 0.0f;
 #pragma unroll
-  for (int i = 0; i < 32; ++i) {
+  for (int i = 0; i < C; ++i) {
     const float s = __shfl_sync(0xffffffffu, xs, i);
-    if (there && c0 + i < rows) *o = from_f32<OT>(static_cast<float>(static_cast<int>(v[i])) * s * ws);
-    o += N;
+    if (there && i < columns) *out = from_f32<OT>(scaled(v[i], s, ws));
+    out += ldo;
   }
 }
 
-template <int CG, typename OT, bool LOADER>
-__global__ void __launch_bounds__(threads(LOADER), 1)
-int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_w, const __grid_constant__ Params p) {
-  static_assert(!(LOADER && CG == 2), "the loader form runs on single SMs");
+__device__ __forceinline__ uint64_t pack2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ float2 unpack2(uint64_t a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
+  return r;
+}
+__device__ __forceinline__ void put2(float* p, int stride, float2 v) { p[0] = v.x; p[stride] = v.y; }
+__device__ __forceinline__ void put2(__half* p, int stride, float2 v) {
+  const __half2 h = __floats2half2_rn(v.x, v.y);
+  p[0] = __low2half(h);
+  p[stride] = __high2half(h);
+}
+__device__ __forceinline__ void put2(__nv_bfloat16* p, int stride, float2 v) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
+  p[0] = __low2bfloat16(h);
+  p[stride] = __high2bfloat16(h);
+}
+
+// A chunk into shared memory, [token][128 channels]: from there 256 (512) consecutive bytes of a token go out together.  (Stored from registers, 64 or 128
+// bytes a warp, a 1024 x 16384 output took 56 us in 16 bits and 32 us in float32, whatever K.)
+template <typename OT, int C>
+__device__ __forceinline__ void stage_chunk(const uint32_t (&v)[C], OT* mine, const float* xs, uint64_t ws2) {
+#pragma unroll
+  for (int i = 0; i < C; i += 4) {
+    const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(xs + i);
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {
+      const uint64_t sum = pack2(static_cast<float>(static_cast<int>(v[i + j])), static_cast<float>(static_cast<int>(v[i + j + 1])));
+      put2(mine + (i + j) * BN, BN, unpack2(mul2(mul2(sum, j == 0 ? s.x : s.y), ws2)));
+    }
+  }
+}
+// The chunk's rows from shared memory, where rows of out do not start on 16 bytes; a group's four warps.
+template <typename OT>
+__device__ __forceinline__ void store_rows(const OT* buf, OT* out, long long ldo, int channels, int columns, int warp, int lane) {
+  for (int row = warp; row < columns; row += 4) {
+    OT* o = out + row * ldo;
+    const OT* src = buf + row * BN;
+    if constexpr (sizeof(OT) == 4) {
+      for (int j = lane; j < channels; j += 32) o[j] = src[j];
+    } else {                                     // pairs on 4 bytes, wherever the row starts
+      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
+      const int head = (reinterpret_cast<uintptr_t>(o) & 2) ? 1 : 0;
+      if (lane == 0 && head && channels > 0) o[0] = src[0];
+      for (int j = head + 2 * lane; j < channels; j += 64) {
+        if (j + 1 < channels) *reinterpret_cast<uint32_t*>(o + j) = h[j] | static_cast<uint32_t>(h[j + 1]) << 16;
+        else o[j] = src[j];
+      }
+    }
+  }
+}
+// A box of out from shared memory; what lies past its last row or column is left out.
+__device__ __forceinline__ void tma_store_2d(const void* tmap, const void* src, int x, int y) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%2, %3}], [%1];\n\t"
+               "cp.async.bulk.commit_group;"
+               ::"l"(tmap), "r"(smem_u32(src)), "r"(x), "r"(y) : "memory");
+}
+__device__ __forceinline__ void tma_stores_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ bool all_epilogue_warps(bool ok) {
+  uint32_t all;
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\t"
+      "bar.red.and.pred q, %2, %3, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+      : "=r"(all) : "r"(ok ? 1u : 0u), "n"(BAR_ALL), "n"(N_EPI * 32) : "memory");
+  return all != 0;
+}
+
+template <int CG, typename OT>
+__global__ void __launch_bounds__(NTHREADS, 1)
+int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_constant__ CUtensorMap tmap_piece, const __grid_constant__ CUtensorMap tmap_w,
+                 const __grid_constant__ CUtensorMap tmap_out, const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem[];
   const Smem L = smem_map(p.bm, CG, p.depth);
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + L.bars);
@@ -275,14 +338,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 
   if (threadIdx.x == 0) {
     // full and empty_d are used in the pair's first CTA only; commits arrive in both
-    for (int i = 0; i < MAX_STAGES; ++i) { mbar_init(&full[i], LOADER ? N_LOADERS : 1); mbar_init(&empty[i], 1); }
-    for (int i = 0; i < 2; ++i) { mbar_init(&full_d[i], 1); mbar_init(&empty_d[i], 4 * CG); }
+    for (int i = 0; i < MAX_STAGES; ++i) { mbar_init(&full[i], 1); mbar_init(&empty[i], 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(&full_d[i], 1); mbar_init(&empty_d[i], N_EPI * CG); }
     mbar_init(drained, 1);
     *flag_abort = 0;
     fence_barrier_init();
     griddep_launch_dependents();
   }
-  if (!LOADER && warp == WARP_TMA && lane == 0) {
+  if (warp == WARP_TMA && lane == 0) {
     tma_prefetch_desc(&tmap_w);
     tma_prefetch_desc(&tmap_x);
     int ahead = p.depth;
@@ -307,25 +370,26 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
 
   if (warp == WARP_TMA) {
     // ------------------------------------------------------------ this CTA's weight rows and tokens of each stage
-    if (!LOADER && lane == 0) {
+    if (lane == 0) {
       griddep_wait();
-      const int rows = p.bm / CG;
       Ring r = {0, 0};
       bool ok = true;
       int issued = 0;
       for (Walk w(p, team); ok && w.next(p);) {
-        const int n0 = w.nt * (CG * BN) + static_cast<int>(crank) * BN, m0 = w.mt * p.bm + static_cast<int>(crank) * rows;
+        const int n0 = w.nt * (CG * BN) + static_cast<int>(crank) * BN, m0 = w.m0 + static_cast<int>(crank) * (w.bm / CG);
+        const int bytes = stage_bytes(w.bm, CG);
+        const CUtensorMap* tmap = w.bm == p.bm ? &tmap_x : &tmap_piece;
         for (int st = w.st0; st < w.st1; ++st, r.step(p.depth)) {
           if (!wait_bar(flag_abort, &empty[r.i], r.phase ^ 1u)) { LCQ_GIVE_UP(60); ok = false; break; }
           uint8_t* dst = smem + r.i * stage;
-          if (crank == 0) mbar_expect_tx(&full[r.i], CG * stage);
+          if (crank == 0) mbar_expect_tx(&full[r.i], CG * bytes);
           if (CG == 2) {
             const uint32_t bar = leader_addr<CG>(full + r.i);
             tma_load_2d_pair(dst, &tmap_w, bar, st * BK, n0);
-            tma_load_2d_pair(dst + W_STAGE, &tmap_x, bar, st * BK, m0);
+            tma_load_2d_pair(dst + W_STAGE, tmap, bar, st * BK, m0);
           } else {
             tma_load_2d(dst, &tmap_w, full + r.i, st * BK, n0);
-            tma_load_2d(dst + W_STAGE, &tmap_x, full + r.i, st * BK, m0);
+            tma_load_2d(dst + W_STAGE, tmap, full + r.i, st * BK, m0);
           }
           ++issued;
         }
@@ -337,13 +401,12 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     // ------------------------------------------------------------ MMA issuer: one warp for the team
     if (crank == 0) {
       const uint32_t desc0 = gemm_tc::make_b_desc(smem_u32(smem));             // descriptors count 16-byte units
-      const uint32_t idesc = make_idesc(p.bm, CG);
       Ring r = {0, 0}, rd = {0, 0};
       bool ok = true;
       for (Walk w(p, team); ok && w.next(p); rd.step(2)) {
         if (!warp_wait(flag_abort, &empty_d[rd.i], rd.phase ^ 1u)) { if (lane == 0) LCQ_GIVE_UP(61); ok = false; break; }
         tc_fence_after();
-        const uint32_t d_t = tmem_base + rd.i * p.bm;
+        const uint32_t d_t = tmem_base + rd.i * p.bm, idesc = make_idesc(w.bm, CG);
         for (int st = w.st0; st < w.st1; ++st, r.step(p.depth)) {
           if (!warp_wait(flag_abort, &full[r.i], r.phase)) { if (lane == 0) LCQ_GIVE_UP(62); ok = false; break; }
           tc_fence_after();
@@ -354,104 +417,77 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         if (ok) umma_commit<CG>(&full_d[rd.i]);
       }
     }
-  } else if (warp < WARP_TMA) {
+  } else if (warp < N_EPI) {
     // ------------------------------------------------------------ epilogue warps: TMEM -> global
     griddep_wait();                            // out and the scratch may still be in the preceding kernel's use
-    const int r = warp * 32 + lane;
-    const uint32_t lane_taddr = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+    constexpr int C = chunk_columns<OT>();
+    const int group = warp >> 2, in_group = warp & 3;
+    const int r = in_group * 32 + lane;        // weight row of the tile = TMEM lane
+    const uint32_t lane_taddr = tmem_base + (static_cast<uint32_t>(in_group * 32) << 16);
     const uint32_t empty_d0 = leader_addr<CG>(empty_d);
-    volatile int* shared_int = flag_abort + FLAG_SHARED;
-    const long long part_elems = static_cast<long long>(p.bm) * BN;
+    const bool stage_out = staged(p.bm);
+    float* xs_tile = reinterpret_cast<float*>(smem + L.xs);
+    uint8_t* buffers = smem + L.out + group * 2 * OUT_BUFFER;
+    int buffer = 0;
+    // The scales of a tile are on their way while the tile before it is stored: fetched in its own turn they showed in every short tile.
+    Walk next(p, team);
+    bool more = next.next(p);
+    float ws_next = 0.0f, xs_next = 0.0f;
+    const auto fetch_scales = [&] {
+      const long long n = static_cast<long long>(next.nt) * (CG * BN) + static_cast<int>(crank) * BN + r;
+      const long long m = static_cast<long long>(next.m0) + static_cast<int>(threadIdx.x);
+      if (n < p.N) ws_next = load_scale(p.w_scales, n, p.w_scale_dtype);
+      if (stage_out && static_cast<int>(threadIdx.x) < next.bm && m < p.M) xs_next = p.x_scales[m];
+    };
+    if (more) fetch_scales();
     Ring rd = {0, 0};
-    for (Walk w(p, team); w.next(p); rd.step(2)) {
-      const int n = w.nt * (CG * BN) + static_cast<int>(crank) * BN + r, m0 = w.mt * p.bm;
+    for (; more; rd.step(2)) {
+      const Walk w = next;
+      const float ws = ws_next;
+      const int n0 = w.nt * (CG * BN) + static_cast<int>(crank) * BN, n = n0 + r, m0 = w.m0;
       const bool there = n < p.N;
       const uint32_t d_t = lane_taddr + rd.i * p.bm;
-      const int rows = p.M - m0 < p.bm ? p.M - m0 : p.bm;
-      const float ws = there ? load_scale(p.w_scales, n, p.w_scale_dtype) : 0.0f;
+      const int rows = p.M - m0 < w.bm ? p.M - m0 : w.bm;
       const float* xs = p.x_scales + m0;
-      OT* out = static_cast<OT*>(p.out) + static_cast<long long>(m0) * p.N + n;
+      OT* out = static_cast<OT*>(p.out) + m0 * p.ldo + n0;
+      if (stage_out) {
+        xs_tile = reinterpret_cast<float*>(smem + L.xs) + rd.i * 256;    // (those of the tile before the last: read by all before the barrier of the last)
+        if (static_cast<int>(threadIdx.x) < w.bm) xs_tile[threadIdx.x] = xs_next;
+      }
+      more = next.next(p);
+      if (more) fetch_scales();
       if (!all_epilogue_warps(wait_bar(flag_abort, &full_d[rd.i], rd.phase))) { if (lane == 0) LCQ_GIVE_UP(63); break; }
       tc_fence_after();
       if (CG == 1 && p.split > 1) break;       // the cluster adds up its shares below
-      // who else contributes to this tile: teams p0 .. p1
-      int p0 = team, p1 = team, slot1 = 0;
-      if (w.tile < p.sk_tiles) {
-        const unsigned t0 = static_cast<unsigned>(w.tile) * static_cast<unsigned>(p.nst);
-        p0 = share_owner(p, t0);
-        p1 = share_owner(p, t0 + static_cast<unsigned>(p.nst) - 1u);
-        slot1 = share_begin(p, p0) < t0;       // p0 came from the tile before (slot 0); the others' shares begin here
-      }
-      const auto part = [&](int q) {
-        return p.partials + (static_cast<long long>(2 * q + (q == p0 ? slot1 : 0)) * CG + crank) * part_elems + r;
-      };
-      bool finish = p1 == p0;
-      int* counter = p.counters + w.tile * CG + crank;
-      if (!finish) {
-        // published already by all the others?  Then this CTA finishes the tile without publishing.
-        if (threadIdx.x == 0) *shared_int = load_acquire(counter);
-        named_bar_sync(BAR_EPI, 128);
-        finish = *shared_int == p1 - p0;
-        named_bar_sync(BAR_EPI, 128);
-        if (!finish) {
-          int* mine = part(team);
-          for (int c0 = 0; c0 < rows; c0 += 32) {
-            uint32_t v[32];
-            tmem_ld32(d_t + c0, v);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (c0 + i < rows) __stcg(mine + (c0 + i) * BN, static_cast<int>(v[i]));
+      for (int c0 = group * C; c0 < rows; c0 += 2 * C) {
+        uint32_t v[C];
+        tmem_load(d_t + c0, v);
+        tmem_wait_ld();
+        const int columns = rows - c0 < C ? rows - c0 : C;
+        if (stage_out) {
+          OT* buf = reinterpret_cast<OT*>(buffers + buffer * OUT_BUFFER);
+          stage_chunk<OT, C>(v, buf + r, xs_tile + c0, pack2(ws, ws));
+          if (p.vec) {
+            fence_async_smem();                // the copy reads through the async proxy
+            if (in_group == 0 && lane == 0) tma_stores_read();        // the copy before this one has left the other buffer, which comes next
+            named_bar_sync(BAR_GROUP + group, 128);
+            if (in_group == 0 && lane == 0 && n0 < p.N) {
+              for (int h = 0; h < columns; h += OUT_BOX) tma_store_2d(&tmap_out, buf + h * BN, n0, m0 + c0 + h);
+            }
+          } else {
+            named_bar_sync(BAR_GROUP + group, 128);
+            store_rows<OT>(buf, out + c0 * p.ldo, p.ldo, p.N - n0 < BN ? p.N - n0 : BN, columns, in_group, lane);
           }
-          __threadfence();
-          named_bar_sync(BAR_EPI, 128);
-          if (threadIdx.x == 0) *shared_int = atomicAdd(counter, 1);
-          named_bar_sync(BAR_EPI, 128);
-          finish = *shared_int == p1 - p0;
-          named_bar_sync(BAR_EPI, 128);
+          buffer ^= 1;
+        } else {
+          store_direct<OT, C>(v, out + r + c0 * p.ldo, p.ldo, there, columns, xs + c0, ws, lane);
         }
-        __threadfence();
-      }
-      if (finish) {
-        for (int c0 = 0; c0 < rows; c0 += 32) {
-          uint32_t v[32];
-          tmem_ld32(d_t + c0, v);
-          tmem_wait_ld();
-          for (int q = p0; q <= p1; ++q) {
-            if (q == team) continue;
-            const int* src = part(q) + c0 * BN;
-            int u[32];
-#pragma unroll
-            for (int i = 0; i < 32; ++i) u[i] = c0 + i < rows ? __ldcg(src + i * BN) : 0;
-#pragma unroll
-            for (int i = 0; i < 32; ++i) v[i] += static_cast<uint32_t>(u[i]);
-          }
-          store_columns<OT>(v, out, p.N, there, c0, rows, xs, ws, lane);
-        }
-        if (p1 != p0 && threadIdx.x == 0) *counter = 0;
       }
       tc_fence_before();
       __syncwarp();
       if (lane == 0) arrive_leader<CG>(empty_d0 + rd.i * 8);
     }
-  } else if (LOADER) {
-    // ------------------------------------------------------------ loader warps: words -> swizzled rows
-    griddep_wait();
-    const int t = threadIdx.x - (WARP_MMA + 1) * 32;
-    Ring r = {0, 0};
-    bool ok = true;
-    for (Walk w(p, team); ok && w.next(p);) {
-      const int n0 = w.nt * BN, m0 = w.mt * p.bm;
-      for (int st = w.st0; st < w.st1; ++st, r.step(p.depth)) {
-        if (!warp_wait(flag_abort, &empty[r.i], r.phase ^ 1u)) { if (lane == 0) LCQ_GIVE_UP(64); ok = false; break; }
-        uint8_t* dst = smem + r.i * stage;
-        load_rows(dst, p.w, p.ldw, n0, BN, p.N - n0, st * BK, p.K, t);
-        load_rows(dst + W_STAGE, p.x, p.ldx, m0, p.bm, p.M - m0, st * BK, p.K, t);
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");           // the MMAs read through the async proxy
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[r.i]);
-      }
-    }
+    if (in_group == 0 && lane == 0) tma_stores_read();      // the buffers outlive the copies
   }
 #undef LCQ_GIVE_UP
 
@@ -459,7 +495,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   __syncthreads();
   if (CG == 2) cluster_barrier();    // neither CTA leaves while the other may still arrive on its barriers or the pair's MMAs read its memory
   if (*flag_abort) {
-    drain<CG, LOADER>(p, smem, crank);
+    drain<CG>(p, smem, team, crank);
     if (CG == 2) cluster_barrier();
   }
   if (CG == 1 && p.split > 1) {
@@ -467,22 +503,22 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     // part of their columns (into the ring, which nobody uses any more).
     Walk w(p, team);
     w.next(p);
-    const int me = team % p.split, m0 = w.mt * p.bm;
+    const int me = team % p.split, m0 = w.m0;
     const int rows = p.M - m0 < p.bm ? p.M - m0 : p.bm;
     const int cw = (rows + p.split - 1) / p.split;
-    const int r = warp * 32 + lane;
+    const int r = (warp & 3) * 32 + lane;
     cluster_barrier();
-    if (warp < WARP_TMA) {
+    if (warp < N_EPI) {
       tc_fence_after();
       const uint32_t mine = smem_u32(smem) + (me * cw * BN + r) * 4;
-      for (int c0 = 0; c0 < rows; c0 += 32) {
-        uint32_t v[32];
-        tmem_ld32(tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + c0, v);
+      for (int c0 = (warp >> 2) * 16; c0 < rows; c0 += 32) {
+        uint32_t v[16];
+        tmem_ld16(tmem_base + (static_cast<uint32_t>((warp & 3) * 32) << 16) + c0, v);
         tmem_wait_ld();
         int d = c0 / cw, j = c0 - d * cw;
         uint32_t dst = peer_addr(mine + j * (BN * 4), d);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
+        for (int i = 0; i < 16; ++i) {
           if (c0 + i < rows) store_remote(dst, static_cast<int>(v[i]));
           dst += BN * 4;
           if (++j == cw && d + 1 < p.split) { j = 0; ++d; dst = peer_addr(mine, d); }
@@ -492,14 +528,14 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
     cluster_barrier();
     const int n = w.nt * BN + r;
-    if (warp < WARP_TMA && n < p.N && *flag_abort == 0) {
+    if (warp < N_EPI && n < p.N && *flag_abort == 0) {
       const int* got = reinterpret_cast<const int*>(smem) + r;
       const float ws = load_scale(p.w_scales, n, p.w_scale_dtype);
-      OT* out = static_cast<OT*>(p.out) + static_cast<long long>(m0 + me * cw) * p.N + n;
-      for (int j = 0; j < cw && me * cw + j < rows; ++j) {
+      OT* out = static_cast<OT*>(p.out) + (m0 + me * cw) * p.ldo + n;
+      for (int j = warp >> 2; j < cw && me * cw + j < rows; j += 2) {
         int sum = 0;
         for (int q = 0; q < p.split; ++q) sum += got[(q * cw + j) * BN];
-        out[static_cast<long long>(j) * p.N] = from_f32<OT>(static_cast<float>(sum) * p.x_scales[m0 + me * cw + j] * ws);
+        out[j * p.ldo] = from_f32<OT>(static_cast<float>(sum) * p.x_scales[m0 + me * cw + j] * ws);
       }
     }
   }
@@ -510,29 +546,92 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   }
 }
 
+// 16 bytes from any address: the two aligned pieces they lie in, and their bytes shifted into place.
+struct Piece {
+  uint4 a, b;
+  int off;
+  // The first `valid` bytes exist (at most 0: none).  Only aligned pieces that hold a byte that exists are read.
+  __device__ __forceinline__ void load(const uint8_t* p, int valid) {
+    off = static_cast<int>(reinterpret_cast<uintptr_t>(p) & 15);
+    const uint4* q = reinterpret_cast<const uint4*>(p - off);
+    a = valid > 0 ? q[0] : make_uint4(0u, 0u, 0u, 0u);
+    b = off + (valid < 16 ? valid : 16) > 16 ? q[1] : make_uint4(0u, 0u, 0u, 0u);
+  }
+  __device__ __forceinline__ uint4 get(int valid) const {
+    uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+    if (off & 8) {
+#pragma unroll
+      for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+      for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    }
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = __funnelshift_r(w[i], w[i + 1], (off & 3) * 8);
+    if (valid < 16) {                          // the end of a row: what follows reads as zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int left = valid - 4 * i;
+        r[i] = left >= 4 ? r[i] : left <= 0 ? 0u : r[i] & ((1u << (8 * left)) - 1u);
+      }
+    }
+    return make_uint4(r[0], r[1], r[2], r[3]);
+  }
+};
+// Rows of K bytes, ld apart, into rows of `per_row` pieces of 16 bytes (the last one filled up with zeros).  total < 2^31 pieces.
+__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* src, long long ld, uint4* dst, int K, int per_row, Divisor by_per_row, int total) {
+  griddep_launch_dependents();
+  griddep_wait();
+  constexpr int EACH = 4;
+  const int stride = static_cast<int>(gridDim.x) * 256;
+  for (long long i0 = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i0 < total; i0 += EACH * stride) {
+    Piece v[EACH];
+    int valid[EACH];
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const long long i = i0 + static_cast<long long>(j) * stride;
+      const int at = i < total ? static_cast<int>(i) : 0;
+      const int row = by_per_row.divide(at), k = (at - row * per_row) * 16;
+      valid[j] = i < total ? K - k : 0;
+      v[j].load(src + row * ld + k, valid[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+      const long long i = i0 + static_cast<long long>(j) * stride;
+      if (i < total) dst[i] = v[j].get(valid[j]);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------- host side
-struct Tiling { int cg, bm, tn, tm, n_tiles, group, teams, sk_tiles, split, depth; };
+struct Tiling { int cg, bm, tn, tm, n_tiles, group, teams, full, tail, split, depth; };
 
 inline int ring_depth(int bm, int cg) {
-  const int fixed = smem_map(bm, cg, 0).total + 1024;
+  const int fixed = smem_map(bm, cg, 0).total;
   const int d = (227 * 1024 - fixed) / stage_bytes(bm, cg);
   return d < MAX_STAGES ? d : MAX_STAGES;
 }
 
-// Clocks of a 128-k stage of a tile: the MMAs (8192 products a clock and SM), the reads of the weight rows from shared memory, and the
-// copies into the ring.
-inline double stage_clocks(int cg, int bm) {
-  const double mma = 2.0 * bm, copies = stage_bytes(bm, cg) / 48.0;
-  const double c = mma > copies ? mma : copies;
-  return c > 140.0 ? c : 140.0;
+// How many clusters of 2 .. 8 CTAs that fill an SM each the GPU holds at once (a cluster stays within a GPC): of 148 SMs as the occupancy
+// query counts them on a B200; other counts of SMs in proportion.
+struct ClusterFit { int n[MAX_SPLIT + 1]; };
+inline ClusterFit cluster_fit(int sm_count) {
+  const int of_148[MAX_SPLIT + 1] = {0, 148, 74, 45, 33, 26, 22, 15, 15};
+  ClusterFit f;
+  for (int c = 0; c <= MAX_SPLIT; ++c) f.n[c] = of_148[c] * sm_count / 148;
+  return f;
 }
 
-inline Tiling choose_tiling(int M, int N, int K, int sm_count, bool loader) {
+// Tile shape, and how the tiles are dealt out: the cheapest form by an estimate in clocks.  Its constants are fitted to 2067 timings, the forms of 110
+// problems of 3 .. 8192 tokens; the forms it chooses take 1 % longer than the fastest on average, a tenth at worst.
+inline Tiling choose_tiling(int M, int N, int K, int sm_count, const ClusterFit& fit) {
   const int nst = (K + BK - 1) / BK;
   Tiling best;
   memset(&best, 0, sizeof(best));
   double best_cost = 1e300;
-  for (int cg = 1; cg <= (loader || sm_count < 2 ? 1 : 2); ++cg) {
+  for (int cg = 1; cg <= (sm_count < 2 ? 1 : 2); ++cg) {
     const int P = sm_count / cg;
     const long long tn = (static_cast<long long>(N) + cg * BN - 1) / (cg * BN);
     const int step = 16 * cg;
@@ -542,43 +641,75 @@ inline Tiling choose_tiling(int M, int N, int K, int sm_count, bool loader) {
       const long long tiles = tn * tm;
       Tiling t;
       t.cg = cg; t.bm = bm; t.tn = static_cast<int>(tn); t.tm = static_cast<int>(tm); t.n_tiles = static_cast<int>(tiles);
-      t.group = bm >= 128 ? 8 : 16;
+      t.group = 8;
       t.depth = ring_depth(bm, cg);
-      const double per = stage_clocks(cg, bm);
-      const auto consider = [&](long long teams, long long sk, int split, double cost) {
-        if (cost >= best_cost) return;
+      // a stage: its MMAs (8192 products a clock and SM, and what power leaves of that), its copies from L2, the hand-over
+      const auto stage = [&](int rows) {
+        const double mma = 2.78 * rows, copies = stage_bytes(rows, cg) / 50.5, c = mma > copies ? mma : copies;
+        return c > 411.0 ? c : 411.0;
+      };
+      // storing a tile: two groups of warps take its 32-column chunks in turn
+      const auto store = [&](int rows) { return 2872.0 + (staged(bm) ? (N % 8 ? 2568.0 : 935.0) * ((rows + 63) / 64) : 0.0); };
+      const auto tile_clocks = [&](int rows) { const double k = nst * stage(rows); return k > store(rows) ? k : store(rows); };
+      const double memory = (static_cast<double>(N) * K + static_cast<double>(M) * K + 2.0 * M * N) / 11424.0;     // at this many bytes a clock from HBM and L2
+      const double start = cg == 1 ? 3279.0 : 6125.0;
+      const auto consider = [&](long long teams, long long full, int tail, int split, double work, double rest) {
+        double used = 1.15 * static_cast<double>(teams) * cg / sm_count;
+        if (used > 1.0) used = 1.0;
+        const double cost = start + (work > memory / used ? work : memory / used) + rest;
+        if (cost > best_cost) return;            // (of equal ones the higher tile)
         best_cost = cost;
-        t.teams = static_cast<int>(teams); t.sk_tiles = static_cast<int>(sk); t.split = split;
+        t.teams = static_cast<int>(teams); t.full = static_cast<int>(full); t.tail = tail; t.split = split;
         best = t;
       };
       const long long waves = tiles / P, rem = tiles % P;
-      const double start = cg == 1 ? 5000.0 : 5600.0;
-      consider(tiles < P ? tiles : P, 0, 1, start + static_cast<double>(waves + (rem != 0)) * nst * per + 10.0 * bm);
+      const long long whole = tiles < P ? tiles : P;
+      consider(whole, tiles, 1, 1, static_cast<double>((tiles + whole - 1) / whole) * tile_clocks(bm), store(bm));
       if (rem == 0) continue;
-      // equal shares of K, with a wave of whole tiles added when the shares would be short
-      const long long sk = rem * 3 >= P || waves == 0 ? rem : rem + P;
-      const long long share = (sk * nst + P - 1) / P;
-      if (nst > 1 && (waves == 0 || sk * nst >= P))       // (every team has a share)
-        consider(P < sk * nst ? P : sk * nst, sk, 1, start + static_cast<double>((tiles - sk) / P) * nst * per + share * per + 3000.0 + 40.0 * bm);
-      if (cg == 1 && waves == 0) {
-        for (int c = 2; c <= MAX_SPLIT && c <= nst; ++c) {
-          if (tiles > static_cast<long long>(sm_count / 18) * (16 / c)) continue;
-          consider(tiles * c, 0, c, start + ((nst + c - 1) / c) * per + 1500.0 + 12.0 * bm);
+      if (waves > 0) {
+        for (int tail = 2; tail <= 8; tail *= 2) {
+          const int piece = bm / tail;
+          if (piece * tail != bm || piece % step != 0) continue;
+          consider(P, tiles - rem, tail, 1, waves * tile_clocks(bm) + static_cast<double>((rem * tail + P - 1) / P) * tile_clocks(piece), store(piece));
         }
+      } else if (cg == 1) {
+        for (int c = 2; c <= MAX_SPLIT && c <= nst; ++c)
+          if (tiles <= fit.n[c]) consider(tiles * c, tiles, 1, c, ((nst + c - 1) / c) * stage(bm), 4984.0 + 75.0 * bm);
       }
     }
   }
   return best;
 }
 
-inline size_t partial_bytes(const Tiling& t) {
-  return t.sk_tiles ? static_cast<size_t>(t.teams) * 2 * t.cg * t.bm * BN * sizeof(int) : 0;
-}
-// [shared counter region][int32 partials of the tiles cut along K]
-inline size_t workspace_bytes(const Tiling& t) { return t.sk_tiles ? kWorkspaceCounterBytes + partial_bytes(t) : 0; }
-
 // Whether TMA can read the operand: rows on 16 bytes.
 inline bool mappable(const void* p, long long ld) { return aligned(p, 16) && ld % 16 == 0; }
+
+// A call: one product, or one for each piece of the weights that are copied first.
+struct Plan {
+  Tiling main, tail;         // of the pieces, and of a last one of fewer rows
+  int piece, tail_rows;      // weight rows of a piece
+  size_t x_copy, w_copy;
+  // [shared counter region][x on 16 bytes][a piece of w on 16 bytes]
+  size_t bytes() const { return x_copy + w_copy ? kWorkspaceCounterBytes + x_copy + w_copy : 0; }
+};
+inline Plan make_plan(int M, int N, int K, int sm_count, const ClusterFit& fit, bool x_mappable, bool w_mappable) {
+  constexpr long long W_COPY = 48ll << 20;     // stays in L2 beside x and out
+  const long long row = (static_cast<long long>(K) + 15) / 16 * 16;
+  Plan q;
+  memset(&q, 0, sizeof(q));
+  q.piece = N;
+  if (!w_mappable && N * row > W_COPY) {
+    const long long pieces = (N * row + W_COPY - 1) / W_COPY, rows = ((N + pieces - 1) / pieces + 255) / 256 * 256;
+    if (rows < N) q.piece = static_cast<int>(rows);
+  }
+  q.tail_rows = N % q.piece;
+  q.main = choose_tiling(M, q.piece, K, sm_count, fit);
+  if (q.tail_rows) q.tail = choose_tiling(M, q.tail_rows, K, sm_count, fit);
+  const auto up = [](long long n) { return static_cast<size_t>((n + 1023) / 1024 * 1024); };
+  if (!x_mappable) q.x_copy = up(M * row);
+  if (!w_mappable) q.w_copy = up(q.piece * row);
+  return q;
+}
 
 inline Params make_params(const Tiling& t, int M, int N, int K) {
   Params p;
@@ -586,15 +717,20 @@ inline Params make_params(const Tiling& t, int M, int N, int K) {
   p.M = M; p.N = N; p.K = K;
   p.bm = t.bm; p.tn = t.tn; p.tm = t.tm; p.n_tiles = t.n_tiles; p.group = t.group;
   p.nst = (K + BK - 1) / BK;
-  p.teams = t.teams; p.sk_tiles = t.sk_tiles; p.split = t.split; p.depth = t.depth;
+  p.teams = t.teams; p.full = t.full; p.tail = t.tail; p.split = t.split; p.depth = t.depth;
+  p.piece_bm = t.bm / t.tail;
+  p.by_tail = make_divisor(t.tail);
+  p.by_group_tiles = make_divisor(t.group * t.tn);
+  p.by_group = make_divisor(t.group);
+  p.by_last_group = make_divisor(t.tm % t.group ? t.tm % t.group : t.group);
   p.tmem_cols = 32;                            // the epilogue reads 32 columns at a time
   while (p.tmem_cols < t.bm + (t.bm + 31) / 32 * 32) p.tmem_cols *= 2;
   return p;
 }
 
-template <int CG, typename OT, bool LOADER>
+template <int CG, typename OT>
 int launch_t(const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
-  auto kern = int8_gemm_kernel<CG, OT, LOADER>;
+  auto kern = int8_gemm_kernel<CG, OT>;
   static thread_local int configured_device = -1;
   int dev = 0;
   LCQ_CUDA_TRY(cudaGetDevice(&dev));
@@ -604,7 +740,7 @@ int launch_t(const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
   }
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  gemm_tc::pdl_launch_config(cfg, attr, CG * p.teams, threads(LOADER), smem_map(p.bm, CG, p.depth).total, stream);
+  gemm_tc::pdl_launch_config(cfg, attr, CG * p.teams, NTHREADS, smem_map(p.bm, CG, p.depth).total, stream);
   const int cluster = CG == 2 ? 2 : p.split;
   if (cluster > 1) {
     cudaLaunchAttribute& a = attr[cfg.numAttrs++];
@@ -613,49 +749,97 @@ int launch_t(const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
     a.val.clusterDim.y = 1;
     a.val.clusterDim.z = 1;
   }
-  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], p));
+  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, kern, tm[0], tm[1], tm[2], tm[3], p));
   return LCQ_OK;
 }
-template <typename OT>
-int launch_by_form(int cg, bool loader, const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
-  if (loader) return launch_t<1, OT, true>(tm, p, stream);
-  return cg == 2 ? launch_t<2, OT, false>(tm, p, stream) : launch_t<1, OT, false>(tm, p, stream);
+
+struct Operands {
+  const void* x; long long ldx;
+  const float* x_scales;
+  const void* w; long long ldw;
+  const void* w_scales; int w_scale_dtype;
+  void* out; long long ldo; int out_dtype;
+};
+// One product of operands that TMA can read.
+inline int launch_tiling(const Tiling& t, const Operands& o, int M, int N, int K, cudaStream_t stream) {
+  Params p = make_params(t, M, N, K);
+  p.out = o.out;
+  p.ldo = o.ldo;
+  p.x_scales = o.x_scales;
+  p.w_scales = o.w_scales;
+  p.w_scale_dtype = o.w_scale_dtype;
+  const int e = o.out_dtype == LCQ_F32 ? 4 : 2;
+  p.vec = aligned(o.out, 16) && (o.ldo * e) % 16 == 0;
+  CUtensorMap tm[4];         // x in whole tiles, x in pieces of a tile, weights, out
+  memset(tm, 0, sizeof(tm));
+  const uint64_t k64 = static_cast<uint64_t>(K), m64 = static_cast<uint64_t>(M), n64 = static_cast<uint64_t>(N);
+  int rc = encode_tmap_2d(&tm[0], 0, o.x, k64, m64, static_cast<uint64_t>(o.ldx), BK, t.bm / t.cg, 3);
+  if (rc != LCQ_OK) return rc;
+  if (t.tail > 1 && (rc = encode_tmap_2d(&tm[1], 0, o.x, k64, m64, static_cast<uint64_t>(o.ldx), BK, t.bm / t.tail / t.cg, 3)) != LCQ_OK) return rc;
+  if ((rc = encode_tmap_2d(&tm[2], 0, o.w, k64, n64, static_cast<uint64_t>(o.ldw), BK, BN, 3)) != LCQ_OK) return rc;
+  if (p.vec && staged(t.bm) && (rc = encode_tmap_2d(&tm[3], e == 4 ? 3 : 1, o.out, n64, m64, static_cast<uint64_t>(o.ldo) * e, BN, OUT_BOX, 0)) != LCQ_OK)
+    return rc;
+  switch (o.out_dtype) {
+    case LCQ_F32: return t.cg == 2 ? launch_t<2, float>(tm, p, stream) : launch_t<1, float>(tm, p, stream);
+    case LCQ_F16: return t.cg == 2 ? launch_t<2, __half>(tm, p, stream) : launch_t<1, __half>(tm, p, stream);
+    case LCQ_BF16: return t.cg == 2 ? launch_t<2, __nv_bfloat16>(tm, p, stream) : launch_t<1, __nv_bfloat16>(tm, p, stream);
+    default: break;
+  }
+  set_error("int8 matmul: bad out_dtype %d", o.out_dtype);
+  return LCQ_ERR_BAD_ARG;
 }
 
-inline int launch_tiling(const Tiling& t, const void* x, long long ldx, const void* x_scales, const void* w, long long ldw, const void* w_scales,
-                         void* out, int M, int N, int K, int w_scale_dtype, int out_dtype, bool loader, void* workspace, size_t ws_bytes,
-                         cudaStream_t stream) {
-  const size_t need = workspace_bytes(t);
+inline int launch_align(const void* src, long long ld, void* dst, long long rows, int K, int sm_count, cudaStream_t stream) {
+  const int per_row = (K + 15) / 16;
+  const long long most = (1ll << 30) / per_row;
+  for (long long r = 0; r < rows; r += most) {
+    const long long n = rows - r < most ? rows - r : most, total = n * per_row;
+    long long blocks = (total + 1023) / 1024;
+    if (blocks > sm_count * 8ll) blocks = sm_count * 8ll;
+    cudaLaunchConfig_t cfg;
+    cudaLaunchAttribute attr[1];
+    gemm_tc::pdl_launch_config(cfg, attr, static_cast<int>(blocks), 256, 0, stream);
+    LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, align_rows_kernel, static_cast<const uint8_t*>(src) + r * ld, ld, static_cast<uint4*>(dst) + r * per_row, K, per_row,
+                                    make_divisor(per_row), static_cast<int>(total)));
+  }
+  return LCQ_OK;
+}
+
+inline int launch(Operands o, int M, int N, int K, void* workspace, size_t ws_bytes, int sm_count, const ClusterFit& fit, cudaStream_t stream) {
+  const bool x_mappable = mappable(o.x, o.ldx), w_mappable = mappable(o.w, o.ldw);
+  const Plan q = make_plan(M, N, K, sm_count, fit, x_mappable, w_mappable);
+  const size_t need = q.bytes();
   if (need && (workspace == nullptr || ws_bytes < need || !aligned(workspace, 256))) {
     set_error("int8 matmul: workspace of %zu bytes (256-byte aligned) required, got %zu", need, ws_bytes);
     return LCQ_ERR_WORKSPACE;
   }
-  Params p = make_params(t, M, N, K);
-  p.out = out;
-  p.x_scales = static_cast<const float*>(x_scales);
-  p.w_scales = w_scales;
-  p.w_scale_dtype = w_scale_dtype;
-  p.x = static_cast<const uint8_t*>(x); p.ldx = ldx;
-  p.w = static_cast<const uint8_t*>(w); p.ldw = ldw;
-  p.counters = static_cast<int*>(workspace);
-  p.partials = need ? reinterpret_cast<int*>(static_cast<uint8_t*>(workspace) + kWorkspaceCounterBytes) : nullptr;
-  CUtensorMap tm[2];
-  memset(tm, 0, sizeof(tm));
-  if (!loader) {
-    const uint64_t k64 = static_cast<uint64_t>(K);
-    // (a single row has no row stride: any multiple of 16 that covers it will do)
-    int rc = encode_tmap_2d(&tm[0], 0, x, k64, static_cast<uint64_t>(M), static_cast<uint64_t>(ldx), BK, t.bm / t.cg, 3);
+  uint8_t* scratch = need ? static_cast<uint8_t*>(workspace) + kWorkspaceCounterBytes : nullptr;
+  const long long row = (static_cast<long long>(K) + 15) / 16 * 16;
+  if (!x_mappable) {
+    const int rc = launch_align(o.x, o.ldx, scratch, M, K, sm_count, stream);
     if (rc != LCQ_OK) return rc;
-    if ((rc = encode_tmap_2d(&tm[1], 0, w, k64, static_cast<uint64_t>(N), static_cast<uint64_t>(ldw), BK, BN, 3)) != LCQ_OK) return rc;
+    o.x = scratch;
+    o.ldx = row;
   }
-  switch (out_dtype) {
-    case LCQ_F32: return launch_by_form<float>(t.cg, loader, tm, p, stream);
-    case LCQ_F16: return launch_by_form<__half>(t.cg, loader, tm, p, stream);
-    case LCQ_BF16: return launch_by_form<__nv_bfloat16>(t.cg, loader, tm, p, stream);
-    default: break;
+  const uint8_t* w = static_cast<const uint8_t*>(o.w);
+  const uint8_t* w_scales = static_cast<const uint8_t*>(o.w_scales);
+  uint8_t* out = static_cast<uint8_t*>(o.out);
+  const long long ldw = o.ldw;
+  for (int n0 = 0; n0 < N; n0 += q.piece) {
+    const int n = N - n0 < q.piece ? N - n0 : q.piece;
+    if (!w_mappable) {
+      const int rc = launch_align(w + n0 * ldw, ldw, scratch + q.x_copy, n, K, sm_count, stream);
+      if (rc != LCQ_OK) return rc;
+      o.w = scratch + q.x_copy;
+      o.ldw = row;
+    }
+    o.w_scales = w_scales + static_cast<size_t>(n0) * (o.w_scale_dtype == LCQ_F32 ? 4 : 2);
+    o.out = out + static_cast<size_t>(n0) * (o.out_dtype == LCQ_F32 ? 4 : 2);
+    const int rc = launch_tiling(n == q.piece ? q.main : q.tail, o, M, n, K, stream);
+    if (rc != LCQ_OK) return rc;
+    if (N - n0 <= q.piece) break;            // (n0 + piece may pass 2^31)
   }
-  set_error("int8 matmul: bad out_dtype %d", out_dtype);
-  return LCQ_ERR_BAD_ARG;
+  return LCQ_OK;
 }
 
 }  // namespace int8_gemm

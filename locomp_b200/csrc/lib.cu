@@ -15,6 +15,7 @@
 #include "quantize.cuh"
 #include "decode_step.cuh"
 #include "int8_gemm.cuh"
+#include "int8_gemv.cuh"
 #include "token_rows.cuh"
 
 namespace lcq {
@@ -60,6 +61,7 @@ int encode_tmap_2d(void* out_map, int dtype_code, const void* base, uint64_t inn
   }
   CUtensorMapDataType dt = dtype_code == 0 ? CU_TENSOR_MAP_DATA_TYPE_UINT8
                           : dtype_code == 1 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                          : dtype_code == 3 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
                                             : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   CUtensorMapSwizzle sw = swizzle_code == 0 ? CU_TENSOR_MAP_SWIZZLE_NONE
                          : swizzle_code == 1 ? CU_TENSOR_MAP_SWIZZLE_32B
@@ -709,6 +711,36 @@ static int check_int8_problem(int M, int N, int K) {
   return LCQ_OK;
 }
 
+// The clusters that the current device holds, asked once; without a device the proportions of a B200.
+static int8_gemm::ClusterFit device_cluster_fit(int sm_count) {
+  using namespace int8_gemm;
+  static std::mutex mu;
+  static ClusterFit known[64];
+  static bool asked[64];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return cluster_fit(sm_count);
+  std::lock_guard<std::mutex> lk(mu);
+  if (!asked[dev]) {
+    known[dev] = cluster_fit(sm_count);
+    const auto kern = int8_gemm_kernel<1, __half>;
+    cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, 227 * 1024);
+    for (int c = 2; c <= MAX_SPLIT; ++c) {
+      cudaLaunchConfig_t cfg;
+      cudaLaunchAttribute attr[2];
+      gemm_tc::pdl_launch_config(cfg, attr, c, NTHREADS, 220 * 1024, nullptr);
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = c;
+      attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+      cfg.numAttrs = 1;
+      int n = 0;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) == cudaSuccess && n >= 0) known[dev].n[c] = n;
+      else cudaGetLastError();
+    }
+    asked[dev] = true;
+  }
+  return known[dev];
+}
+
 int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, void* out,
                     int M, int N, int K, int w_scale_dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream) {
   int rc = check_int8_problem(M, N, K);
@@ -723,77 +755,72 @@ int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void
   if (di.major != 10) { set_error("tensor-core kernels are built for sm_100a only; device is sm_%d%d", di.major, di.minor); return LCQ_ERR_UNSUPPORTED; }
   ldx = stride_of(M, ldx, K);
   ldw = stride_of(N, ldw, K);
-  const bool loader = !int8_gemm::mappable(x, ldx) || !int8_gemm::mappable(w, ldw);
-  return int8_gemm::launch_tiling(int8_gemm::choose_tiling(M, N, K, di.sm_count, loader), x, ldx, x_scales, w, ldw, w_scales, out, M, N, K,
-                                  w_scale_dtype, out_dtype, loader, workspace, workspace_bytes, static_cast<cudaStream_t>(stream));
+  int8_gemm::Operands o = {};
+  o.x = x; o.ldx = ldx;
+  o.x_scales = static_cast<const float*>(x_scales);
+  o.w = w; o.ldw = ldw;
+  o.w_scales = w_scales; o.w_scale_dtype = w_scale_dtype;
+  o.out = out; o.ldo = N; o.out_dtype = out_dtype;
+  if (int8_gemv::takes(M, N, K, int8_gemm::mappable(x, ldx) && int8_gemm::mappable(w, ldw))) return int8_gemv::launch(o, M, N, K, static_cast<cudaStream_t>(stream));
+  return int8_gemm::launch(o, M, N, K, workspace, workspace_bytes, di.sm_count, device_cluster_fit(di.sm_count), static_cast<cudaStream_t>(stream));
 }
 
-size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K) {
+size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K, int x_on_16, int w_on_16) {
   if (check_int8_problem(M, N, K) != LCQ_OK) return static_cast<size_t>(-1);
-  if (M == 0 || N == 0) return 0;
+  if (M == 0 || N == 0 || int8_gemv::takes(M, N, K, x_on_16 && w_on_16)) return 0;
   int sm = 148, dev = 0, v = 0;
   if (cudaGetDevice(&dev) == cudaSuccess && cudaDeviceGetAttribute(&v, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess && v > 0) sm = v;
-  const size_t a = int8_gemm::workspace_bytes(int8_gemm::choose_tiling(M, N, K, sm, false));
-  const size_t b = int8_gemm::workspace_bytes(int8_gemm::choose_tiling(M, N, K, sm, true));
-  return a > b ? a : b;
+  return int8_gemm::make_plan(M, N, K, sm, device_cluster_fit(sm), x_on_16 != 0, w_on_16 != 0).bytes();
 }
 
-// Replays the schedule of all teams: every (tile, stage) once, contributors and slots of the cut tiles as the kernel derives them.
-int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int aligned_rows, int* fields) {
+// Replays the schedule of all teams: every output and every stage of it once.
+static int check_int8_tiling(const int8_gemm::Tiling& t, int M, int N, int K, int sm_count) {
+  using namespace int8_gemm;
+  const Params p = make_params(t, M, N, K);
+  const int smem = smem_map(p.bm, t.cg, p.depth).total;
+  const auto wrong = [](const char* what) { set_error("int8 plan: %s", what); return LCQ_ERR_BAD_ARG; };
+  if (smem > 227 * 1024 || t.depth < 2 || t.depth > MAX_STAGES) return wrong("shared memory");
+  if (t.bm % (16 * t.cg) != 0 || t.bm > 256 || p.tmem_cols > 512 || t.bm + (t.bm + 31) / 32 * 32 > p.tmem_cols) return wrong("tensor memory");
+  if (t.tail < 1 || p.piece_bm * t.tail != t.bm || p.piece_bm % (16 * t.cg) != 0 || t.full > t.n_tiles || (t.full < t.n_tiles && t.tail == 1) || (t.split > 1 && t.tail > 1))
+    return wrong("pieces of tiles");
+  if (t.split > 1 && (t.cg != 1 || t.teams != t.n_tiles * t.split || ((p.M < p.bm ? p.M : p.bm) + t.split - 1) / t.split * t.split * BN * 4 > t.depth * stage_bytes(p.bm, 1)))
+    return wrong("cluster");
+  if (t.split == 1 && t.cg * t.teams > sm_count) return wrong("more CTAs than SMs");
+  const int unit = 16, units = (M + unit - 1) / unit;                     // of tokens
+  std::vector<int> stages(static_cast<size_t>(units) * t.tn, 0);          // stages of K that each unit of each channel tile has had
+  for (int team = 0; team < t.teams; ++team) {
+    int items = 0;
+    for (Walk w(p, team); w.next(p); ++items) {
+      if (w.tile < 0 || w.tile >= t.n_tiles || w.st0 < 0 || w.st1 > p.nst || w.st0 >= w.st1) return wrong("segment out of range");
+      if (w.nt < 0 || w.nt >= t.tn || w.mt < 0 || w.mt >= t.tm || w.m0 % unit != 0 || w.m0 < w.mt * p.bm || w.m0 + w.bm > (w.mt + 1) * p.bm || w.m0 >= M)
+        return wrong("tile out of place");
+      for (int u = w.m0 / unit; u < (w.m0 + w.bm) / unit && u < units; ++u) stages[static_cast<size_t>(u) * t.tn + w.nt] += w.st1 - w.st0;
+      if (t.split > 1 && items > 0) return wrong("two tiles in a cluster");
+    }
+  }
+  for (int s : stages)
+    if (s != p.nst) return wrong("stages left out or twice");
+  return LCQ_OK;
+}
+
+int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int w_on_16, int* fields) {
   using namespace int8_gemm;
   int rc = check_int8_problem(M, N, K);
   if (rc != LCQ_OK) return rc;
   if (M == 0 || N == 0 || sm_count <= 0) { set_error("int8 plan: nothing to plan"); return LCQ_ERR_BAD_ARG; }
-  const Tiling t = choose_tiling(M, N, K, sm_count, !aligned_rows);
-  const Params p = make_params(t, M, N, K);
-  const int smem = smem_map(p.bm, t.cg, p.depth).total;
+  const Plan q = make_plan(M, N, K, sm_count, cluster_fit(sm_count), true, w_on_16 != 0);
+  const auto wrong = [](const char* what) { set_error("int8 plan: %s", what); return LCQ_ERR_BAD_ARG; };
+  if (q.piece <= 0 || q.tail_rows != N % q.piece || (q.piece < N && q.piece % 256 != 0)) return wrong("pieces of the weights");
+  if (q.tail_rows) {
+    rc = check_int8_tiling(q.tail, M, q.tail_rows, K, sm_count);
+    if (rc != LCQ_OK) return rc;
+  }
   if (fields) {
-    const int f[8] = {t.cg * t.teams, t.bm, t.n_tiles, t.sk_tiles, smem, t.cg, t.split, t.depth};
+    const Tiling& t = q.main;
+    const int f[9] = {t.cg * t.teams, t.bm, t.n_tiles, t.tail > 1 ? t.n_tiles - t.full : 0, smem_map(t.bm, t.cg, t.depth).total, t.cg, t.split, t.depth, q.piece};
     memcpy(fields, f, sizeof(f));
   }
-  const auto wrong = [](const char* what) { set_error("int8 plan: %s", what); return LCQ_ERR_BAD_ARG; };
-  if (smem > 227 * 1024 || t.depth < 2 || t.depth > MAX_STAGES) return wrong("shared memory");
-  if (t.bm % (16 * t.cg) != 0 || t.bm > 256 || p.tmem_cols > 512 || t.bm + (t.bm + 31) / 32 * 32 > p.tmem_cols) return wrong("tensor memory");
-  if (static_cast<size_t>(t.sk_tiles) * t.cg * sizeof(int) > kWorkspaceCounterBytes) return wrong("counters");
-  if (t.split > 1 && (t.cg != 1 || t.teams != t.n_tiles * t.split || (p.bm + t.split - 1) / t.split * t.split * BN * 4 > t.depth * stage_bytes(p.bm, 1)))
-    return wrong("cluster");
-  if (t.split == 1 && t.cg * t.teams > sm_count) return wrong("more CTAs than SMs");
-  std::vector<uint8_t> seen(static_cast<size_t>(t.n_tiles) * p.nst), place(static_cast<size_t>(t.tn) * t.tm);
-  std::vector<int> contributors(t.sk_tiles, 0);
-  std::vector<int> slot_tile(static_cast<size_t>(t.teams) * 2, -1);
-  for (int team = 0; team < t.teams; ++team) {
-    int last_tile = -1;
-    for (Walk w(p, team); w.next(p);) {
-      if (w.tile < 0 || w.tile >= t.n_tiles || w.st0 < 0 || w.st1 > p.nst || w.st0 >= w.st1) return wrong("segment out of range");
-      if (w.nt < 0 || w.nt >= t.tn || w.mt < 0 || w.mt >= t.tm) return wrong("tile out of place");
-      if (w.st0 == 0) {
-        if (place[static_cast<size_t>(w.mt) * t.tn + w.nt]++) return wrong("two tiles in one place");
-      }
-      for (int st = w.st0; st < w.st1; ++st)
-        if (seen[static_cast<size_t>(w.tile) * p.nst + st]++) return wrong("a stage twice");
-      if (w.tile < p.sk_tiles) {
-        const unsigned t0 = static_cast<unsigned>(w.tile) * static_cast<unsigned>(p.nst);
-        const int p0 = share_owner(p, t0), p1 = share_owner(p, t0 + static_cast<unsigned>(p.nst) - 1u);
-        if (team < p0 || team > p1) return wrong("contributor out of range");
-        ++contributors[w.tile];
-        if (p1 != p0) {
-          const int slot = team == p0 && share_begin(p, p0) < t0;
-          int& holds = slot_tile[static_cast<size_t>(team) * 2 + slot];
-          if (holds >= 0) return wrong("a slot twice");
-          holds = w.tile;
-        }
-      }
-      if (w.tile == last_tile) return wrong("a tile twice in one team");
-      last_tile = w.tile;
-    }
-  }
-  for (uint8_t s : seen) if (s != 1) return wrong("a stage left out");
-  for (uint8_t s : place) if (s != 1) return wrong("a place left out");
-  for (int i = 0; i < t.sk_tiles; ++i) {
-    const unsigned t0 = static_cast<unsigned>(i) * static_cast<unsigned>(p.nst);
-    if (contributors[i] != share_owner(p, t0 + static_cast<unsigned>(p.nst) - 1u) - share_owner(p, t0) + 1) return wrong("contributors of a cut tile");
-  }
-  return LCQ_OK;
+  return check_int8_tiling(q.main, M, q.piece, K, sm_count);
 }
 
 static int check_rows(const char* what, int64_t rows, int n) {

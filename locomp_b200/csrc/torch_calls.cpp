@@ -507,7 +507,8 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     rc = call(scratch.ptr, scratch.bytes);
     if (rc == LCQ_ERR_WORKSPACE) {
       released.end();
-      const size_t need = api.int8_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K));
+      const auto on_16 = [](const void* rows, int64_t n, int64_t ld) { return reinterpret_cast<uintptr_t>(rows) % 16 == 0 && (n == 1 || ld % 16 == 0); };
+      const size_t need = api.int8_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), on_16(xp, M, ldx), on_16(wp, N, ldw));
       PyObject* r = PyObject_CallFunction(make_workspace, "niK", static_cast<Py_ssize_t>(need), dev,
                                           static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)));
       if (!r) return nullptr;

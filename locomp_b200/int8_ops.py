@@ -229,17 +229,15 @@ def residual_norms(hidden, delta, weight=None, eps: float = 1e-5, *, post_weight
 
 
 # ------------------------------------------------------------------------------------------ the product
-_CAPTURE_COUNTER_BYTES = 4096          # more than one counter for each tile that is cut along K, of which there are at most twice as many as SMs
-
-
 def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] = None, stream=None,
                 workspace_buf: Optional[torch.Tensor] = None):
     """out[m, n] = (sum_k x[m, k] * w[n, k]) * x_scales[m] * w_scales[n]: an exact integer sum, scaled in float32 and rounded once.
 
     x: int8 [K] or [M, K]; x_scales: float32, M values; w: int8 [N, K]; w_scales: N values (f32 / f16 / bf16).  Rows of x and w may be
-    further apart than K.  Returns a torch CUDA tensor [N] or [M, N] of out_dtype ("f32", "f16", "bf16"; default "f16") or `out`.
-    K is at most 131071.  Scratch as for quantized_matmul (one buffer per stream); under CUDA-graph capture a call without workspace_buf
-    allocates its scratch in the graph's own memory, so that no two graphs share it."""
+    further apart than K; those that do not start on 16 bytes (K % 16 != 0 in contiguous storage) cost a copy.
+    Returns a torch CUDA tensor [N] or [M, N] of out_dtype ("f32", "f16", "bf16"; default "f16") or `out`.  K is at most 131071.
+    Scratch is needed for such copies only: workspace_buf, or this package's buffer of the stream; under CUDA-graph capture the graph's own memory,
+    so that no two graphs share it."""
     if isinstance(x, torch.Tensor) and stream is None:
         res = _lib.calls.int8_matmul(x, x_scales, w, w_scales, out, -1 if out_dtype is None else KIND_TO_CODE.get(out_dtype, -2), workspace_buf)
         if res is not NotImplemented:
@@ -278,7 +276,7 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
         if oo.device != dev:
             raise ValueError("all operands must live on one device")
         sp = current_stream_ptr()
-        need = L.lcq_int8_matmul_workspace_bytes(M, N, K)
+        need = L.lcq_int8_matmul_workspace_bytes(M, N, K, _on_16(xo, M, ldx), _on_16(wo, N, ldw))
         if need == (1 << 64) - 1:
             _lib.check(L.lcq_int8_matmul(xo.ptr, ldx, xso.ptr, wo.ptr, ldw, wso.ptr, oo.ptr, M, N, K, sk, ok, None, 0, sp))    # raises
 
@@ -292,9 +290,7 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
                 raise ValueError(f"workspace_buf must hold {need} bytes on cuda:{dev}")
             launch(workspace_buf)
         elif torch.cuda.is_current_stream_capturing():
-            own = torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev))
-            own[:_CAPTURE_COUNTER_BYTES].zero_()
-            launch(own)
+            launch(torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev)))
         else:
             with locked_workspace(dev, sp):
                 launch(workspace(need, dev, sp))
@@ -303,9 +299,14 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
     return res[0] if out is None and squeeze else res
 
 
-def int8_matmul_workspace_bytes(M: int, N: int, K: int) -> int:
-    """Scratch bytes int8_matmul needs for this problem (0 if none)."""
-    n = _lib.lib().lcq_int8_matmul_workspace_bytes(M, N, K)
+def _on_16(op: Operand, rows: int, ld: int) -> bool:
+    return rows == 0 or (op.ptr % 16 == 0 and (rows == 1 or ld % 16 == 0))
+
+
+def int8_matmul_workspace_bytes(M: int, N: int, K: int, x_on_16: bool = True, w_on_16: bool = True) -> int:
+    """Scratch bytes int8_matmul needs for this problem (0 if none).  x_on_16, w_on_16: whether rows of x and of w start on 16 bytes, as those
+    of QuantizedTokens and Int8Linear do; any other are copied into the scratch first (x whole, w at most 48 MiB at a time)."""
+    n = _lib.lib().lcq_int8_matmul_workspace_bytes(M, N, K, x_on_16, w_on_16)
     if n == (1 << 64) - 1:
         raise ValueError("no kernel covers this problem")
     return int(n)

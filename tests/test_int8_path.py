@@ -35,9 +35,9 @@ def status_ok():
 
 # ------------------------------------------------------------------------------------------ the product's schedule (CPU)
 def plan(m, n, k, sms=148, aligned=1):
-    f = (ctypes.c_int * 8)()
+    f = (ctypes.c_int * 9)()
     assert _lib.lib().lcq_int8_matmul_plan_check(m, n, k, sms, aligned, f) == 0, (m, n, k, sms, aligned, _lib.lib().lcq_last_error())
-    return dict(zip(("ctas", "bm", "tiles", "cut", "smem", "cg", "split", "depth"), f))
+    return dict(zip(("ctas", "bm", "tiles", "in_pieces", "smem", "cg", "split", "depth", "piece"), f))
 
 
 def test_plan_covers_every_stage_once():
@@ -53,13 +53,13 @@ def test_plan_covers_every_stage_once():
 
 
 def test_plan_refuses_what_the_product_refuses():
-    lib, f = _lib.lib(), (ctypes.c_int * 8)()
+    lib, f = _lib.lib(), (ctypes.c_int * 9)()
     assert lib.lcq_int8_matmul_plan_check(1, 1, 131071, 148, 1, f) == 0
     assert lib.lcq_int8_matmul_plan_check(1, 1, 131072, 148, 1, f) == _lib.ERR_UNSUPPORTED
     assert lib.lcq_int8_matmul_plan_check(1, 1, 0, 148, 1, f) == _lib.ERR_BAD_ARG
     assert lib.lcq_int8_matmul_plan_check(2000000000, 2000000000, 64, 148, 1, f) == _lib.ERR_UNSUPPORTED
-    assert lib.lcq_int8_matmul_workspace_bytes(1, 1, 131072) == (1 << 64) - 1 == lib.lcq_int8_matmul_workspace_bytes(-1, 1, 64)
-    assert lib.lcq_int8_matmul_workspace_bytes(0, 1, 64) == 0
+    assert lib.lcq_int8_matmul_workspace_bytes(1, 1, 131072, 1, 1) == (1 << 64) - 1 == lib.lcq_int8_matmul_workspace_bytes(-1, 1, 64, 1, 1)
+    assert lib.lcq_int8_matmul_workspace_bytes(0, 1, 64, 1, 1) == 0
     with pytest.raises(ValueError):
         int8_matmul_workspace_bytes(1, 1, 1 << 20)
 
@@ -132,7 +132,7 @@ def check_product(y, ref, kind):
 PRODUCTS = [(1, 1, 1), (1, 128, 128), (1, 2048, 2048), (2, 130, 64), (3, 5, 16), (16, 28672, 1024), (17, 129, 144), (1, 49152, 576), (5, 4096, 14336),
             (31, 257, 1040), (32, 1000, 576), (33, 300, 512), (64, 5000, 4096), (100, 77, 2064), (128, 512, 4096), (255, 384, 272), (256, 2048, 4096),
             (257, 1001, 1024), (512, 9000, 768), (1000, 2048, 8192), (1025, 513, 640), (2049, 3000, 256), (4096, 128, 1024), (700, 20000, 512)]
-UNALIGNED = [(1, 1, 7), (1, 300, 100), (5, 200, 333), (333, 1003, 1032), (64, 1000, 577), (1, 9000, 577), (200, 300, 17), (129, 130, 1), (16, 3000, 4104), (600, 700, 2049)]
+UNALIGNED = [(1, 1, 7), (1, 300, 100), (5, 200, 333), (333, 1003, 1032), (64, 1000, 577), (1, 9000, 577), (200, 300, 17), (129, 130, 1), (16, 3000, 4104), (600, 700, 2049), (3, 50001, 1001), (40, 14000, 4099)]
 
 
 @pytest.mark.gpu
@@ -239,8 +239,9 @@ def test_product_on_other_streams_and_threads():
 @pytest.mark.gpu
 def test_graphs_do_not_share_scratch():
     """Two captured products that need scratch, replayed beside one another on two streams."""
-    shapes = [(m, n, 4096) for m in (16, 300) for n in range(2000, 30000, 1000) if int8_matmul_workspace_bytes(m, n, 4096)]
-    cases = [product_case(*shapes[0]), product_case(*shapes[-1])]
+    shapes = [(16, 9000, 4100), (300, 5000, 2001)]                         # rows off 16 bytes
+    assert all(int8_matmul_workspace_bytes(*s, False, False) > int8_matmul_workspace_bytes(*s) == 0 for s in shapes)
+    cases = [product_case(*s) for s in shapes]
     graphs, outs = [], []
     for c in cases:
         L.int8_matmul(*c[:4], out_dtype="f32")
@@ -262,7 +263,7 @@ def test_graphs_do_not_share_scratch():
         torch.cuda.synchronize()
         for y, c in zip(outs, cases):
             check_product(y, c[4], torch.float32)
-    ws = torch.zeros(int8_matmul_workspace_bytes(*shapes[0]), dtype=torch.uint8, device="cuda")
+    ws = torch.zeros(int8_matmul_workspace_bytes(*shapes[0], False, False), dtype=torch.uint8, device="cuda")
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
         y = L.int8_matmul(*cases[0][:4], out_dtype="f32", workspace_buf=ws)
@@ -274,9 +275,8 @@ def test_graphs_do_not_share_scratch():
 
 @pytest.mark.gpu
 def test_product_shares_scratch_with_the_int4_product():
-    """One buffer a stream: both leave its counters at zero."""
-    n = next(n for n in range(2000, 30000, 1000) if int8_matmul_workspace_bytes(16, n, 4096))
-    x, xs, w, ws, ref = product_case(16, n, 4096)
+    """One buffer a stream: the int8 product leaves the counters alone that the int4 product wants at zero."""
+    x, xs, w, ws, ref = product_case(16, 9000, 4101)
     g = gen(3)
     w4 = torch.randint(0, 256, (20000, 2048), dtype=torch.uint8, device="cuda", generator=g)
     s4 = (torch.rand(20000, 128, device="cuda", generator=g) * 0.02).half()
@@ -318,7 +318,7 @@ def test_product_refusals():
         L.int8_matmul(x, xs, w, ws, out_dtype="i8")
     with pytest.raises(ValueError, match="must be \\[K\\]"):
         L.int8_matmul(x.view(2, 2, 64), xs, w, ws)
-    big = product_case(16, next(n for n in range(2000, 30000, 1000) if int8_matmul_workspace_bytes(16, n, 4096)), 4096)
+    big = product_case(16, 5000, 1001)
     with pytest.raises(ValueError, match="workspace_buf"):
         L.int8_matmul(*big[:4], workspace_buf=torch.zeros(256, dtype=torch.uint8, device="cuda"))
     assert L.int8_matmul(x[:0], xs[:0], w, ws).shape == (0, 40)
