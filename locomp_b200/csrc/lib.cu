@@ -842,8 +842,12 @@ int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q,
   a.out = q; a.ldo = stride_of(rows, ldq, n);
   a.scales = static_cast<float*>(scales);
   a.n_rows = rows; a.n = n; a.eps = eps;
+  DevInfo di;
+  rc = current_dev_info(di);
+  if (rc != LCQ_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::ROWS, true>(a, st)))
+  if (weight) { LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::NORM_ROWS, true>(a, di.sm_count, st))) }
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::ROWS, true>(a, di.sm_count, st)))
 }
 
 int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* q, int64_t ldq, void* scales, int64_t rows,
@@ -859,8 +863,11 @@ int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64
   a.out = q; a.ldo = stride_of(rows, ldq, n);
   a.scales = static_cast<float*>(scales);
   a.n_rows = rows; a.n = n;
+  DevInfo di;
+  rc = current_dev_info(di);
+  if (rc != LCQ_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::SILU_MUL, true>(a, st)))
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::SILU_MUL, true>(a, di.sm_count, st)))
 }
 
 int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
@@ -885,9 +892,12 @@ int lcq_residual_norms(const void* hidden, const void* delta, const void* post_w
   a.out = weight ? out : nullptr; a.ldo = weight ? stride_of(rows, ld_out, n) : 0;
   a.scales = static_cast<float*>(scales);
   a.n_rows = rows; a.n = n; a.eps = eps; a.scale = scale;
+  DevInfo di;
+  rc = current_dev_info(di);
+  if (rc != LCQ_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (scales) { LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, true>(a, st))) }
-  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, false>(a, st)))
+  if (scales) { LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, true>(a, di.sm_count, st))) }
+  LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, false>(a, di.sm_count, st)))
 }
 
 // ---------------------------------------------------------------- one kernel per decode step

@@ -12,9 +12,11 @@
 // With one, the factor rsqrt(..) is common to v and s: q is taken from the products with the weight alone, and one reduction finds
 // their maximum together with the sum of squares.
 //
-// HBM-bound; each value is read once and kept in registers from the first load to the last use.  A row belongs to a block of
-// as many threads as it has groups of E octets, or to a warp where it is short; all of a thread's loads are issued before the
-// first reduction.  Rows longer than a block holds are walked in chunks and read again (from L2) for each pass over them.
+// HBM-bound; each value is read once and kept in registers from the first load to the last use.  A row belongs to a block of as many threads as
+// it has groups of E octets (8 consecutive values), or to a warp where it is short; all of a thread's loads are issued before the first reduction.
+// Rows longer than a block holds are walked in chunks and read again (from L2) for each pass over them.
+// ALIGNED = false: rows start anywhere and have any length.  Octets then begin where the row that is written lies on 16 bytes, so that only the first and the last
+// one are stored value by value; what is read lies in two (float32: three) aligned pieces, whose values are shifted into place.
 #pragma once
 #include "common.cuh"
 #include "glue.cuh"
@@ -23,12 +25,12 @@
 namespace lcq {
 namespace rows {
 
-enum Op { ROWS, SILU_MUL, RESIDUAL };
+enum Op { ROWS, NORM_ROWS, SILU_MUL, RESIDUAL };
 
 struct Args {
-  const void *a, *b;           // ROWS: x; SILU_MUL: gate, up; RESIDUAL: hidden, delta
+  const void *a, *b;           // ROWS, NORM_ROWS: x; SILU_MUL: gate, up; RESIDUAL: hidden, delta
   long long lda, ldb;          // elements between rows
-  const void* weight;          // RESIDUAL, and ROWS with a norm
+  const void* weight;          // NORM_ROWS; RESIDUAL: may be null
   const void* post_weight;     // RESIDUAL: may be null
   const void* gate;            // RESIDUAL: may be null; [gate_rows, n]
   long long rows_per_gate;
@@ -41,273 +43,365 @@ struct Args {
   float eps, scale;
 };
 
-// Eight values of a row as they are stored: consecutive ones (VEC), or every `step`-th.
-template <typename T, bool VEC> struct Octet;
-template <typename T> struct Octet<T, true> {
-  uint4 r[sizeof(T) / 2];
-  __device__ __forceinline__ void load(const T* p, int, int) {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r[i] = reinterpret_cast<const uint4*>(p)[i];
-  }
-  __device__ __forceinline__ void zero() {
-#pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) r[i] = make_uint4(0u, 0u, 0u, 0u);
-  }
+// Eight values as they are stored.
+template <typename T> struct Octet {
+  static constexpr int W = sizeof(T) / 2;            // 16-byte pieces
+  uint4 r[W];
   __device__ __forceinline__ void get(float (&v)[8]) const { glue::load_vec8<T>(reinterpret_cast<const T*>(r), v); }
   __device__ __forceinline__ void set(const float (&v)[8]) { glue::store_vec8<T>(reinterpret_cast<T*>(r), v); }
-  __device__ __forceinline__ void store(T* p, int, int) const {
+  // Values i .. i + 7 of a row of n, those there are.
+  template <bool ALIGNED> __device__ __forceinline__ void store(T* row, int i, int n) const {
+    T* p = row + i;
+    if (ALIGNED || (i >= 0 && i + 8 <= n && (reinterpret_cast<uintptr_t>(p) & 15) == 0)) {
 #pragma unroll
-    for (int i = 0; i < static_cast<int>(sizeof(T) / 2); ++i) reinterpret_cast<uint4*>(p)[i] = r[i];
+      for (int j = 0; j < W; ++j) reinterpret_cast<uint4*>(p)[j] = r[j];
+    } else {
+      float v[8];
+      get(v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (i + j >= 0 && i + j < n) p[j] = from_f32<T>(v[j]);
+    }
   }
 };
-template <typename T> struct Octet<T, false> {
-  T r[8];
-  __device__ __forceinline__ void load(const T* p, int step, int left) {      // left: values from p on that exist
+// The same on their way from memory: the aligned pieces they lie in.
+template <typename T, bool ALIGNED> struct Raw {
+  static constexpr int W = Octet<T>::W;
+  uint4 r[W];
+  __device__ __forceinline__ void load(const T* row, int i, int) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = j * step < left ? p[j * step] : from_f32<T>(0.0f);
+    for (int j = 0; j < W; ++j) r[j] = reinterpret_cast<const uint4*>(row + i)[j];
   }
-  __device__ __forceinline__ void zero() {
+  __device__ __forceinline__ Octet<T> octet(const T*, int, int) const {
+    Octet<T> o;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = from_f32<T>(0.0f);
+    for (int j = 0; j < W; ++j) o.r[j] = r[j];
+    return o;
   }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
+};
+template <typename T> struct Raw<T, false> {
+  static constexpr int W = Octet<T>::W, S = sizeof(T);
+  uint4 r[W + 1];
+  // Only pieces that hold one of the values 0 .. n - 1 are read.
+  __device__ __forceinline__ void load(const T* row, int i, int n) {
+    const uintptr_t p = reinterpret_cast<uintptr_t>(row) + static_cast<long long>(i) * S;
+    const int off = static_cast<int>(p & 15);
+    const int first = off + (i < 0 ? -i : 0) * S, end = off + (n - i < 8 ? n - i : 8) * S;
+    const uint4* q = reinterpret_cast<const uint4*>(p - off);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(r[j]);
+    for (int j = 0; j <= W; ++j) r[j] = 16 * j < end && 16 * (j + 1) > first ? q[j] : make_uint4(0u, 0u, 0u, 0u);
   }
-  __device__ __forceinline__ void set(const float (&v)[8]) {
+  // The values in place; those that do not exist are zero.
+  __device__ __forceinline__ Octet<T> octet(const T* row, int i, int n) const {
+    const int off = static_cast<int>((reinterpret_cast<uintptr_t>(row) + static_cast<long long>(i) * S) & 15);
+    uint32_t w[4 * W + 4];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) r[j] = from_f32<T>(v[j]);
-  }
-  __device__ __forceinline__ void store(T* p, int step, int left) const {
+    for (int j = 0; j <= W; ++j) { w[4 * j] = r[j].x; w[4 * j + 1] = r[j].y; w[4 * j + 2] = r[j].z; w[4 * j + 3] = r[j].w; }
+    if (off & 8) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (j * step < left) p[j * step] = r[j];
+      for (int j = 0; j < 4 * W + 2; ++j) w[j] = w[j + 2];
+    }
+    if (off & 4) {
+#pragma unroll
+      for (int j = 0; j < 4 * W + 1; ++j) w[j] = w[j + 1];
+    }
+    if (S == 2) {
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 2) * 8);
+    }
+    if (i < 0 || i + 8 > n) {
+#pragma unroll
+      for (int j = 0; j < 4 * W; ++j) {
+        const int k = i + j * (4 / S);               // the word's first value
+        uint32_t keep = S == 4 ? (k >= 0 && k < n ? 0xFFFFFFFFu : 0u) : (k >= 0 && k < n ? 0xFFFFu : 0u) | (k + 1 >= 0 && k + 1 < n ? 0xFFFF0000u : 0u);
+        w[j] &= keep;
+      }
+    }
+    Octet<T> o;
+#pragma unroll
+    for (int j = 0; j < W; ++j) o.r[j] = make_uint4(w[4 * j], w[4 * j + 1], w[4 * j + 2], w[4 * j + 3]);
+    return o;
   }
 };
 
-// Sum of s and maximum of m (bits of a magnitude: NaN above infinity above the numbers) over the threads of a row.
+// The larger magnitude, or NaN where there is one.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Sum of s and maximum of m over the threads of a row.
 template <bool WARP_ROW>
-__device__ __forceinline__ void reduce_row(float& s, uint32_t& m, float2* red) {
+__device__ __forceinline__ void reduce_row(float& s, float& m, float2* red) {
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, off);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
   }
   if (WARP_ROW) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, nw = blockDim.x >> 5;
-  if (lane == 0) red[warp] = make_float2(s, __uint_as_float(m));
+  if (lane == 0) red[warp] = make_float2(s, m);
   __syncthreads();
   const float2 t = lane < nw ? red[lane] : make_float2(0.0f, 0.0f);
   s = t.x;
-  m = __float_as_uint(t.y);
+  m = t.y;
 #pragma unroll
   for (int off = 16; off > 0; off >>= 1) {
     s += __shfl_xor_sync(0xffffffffu, s, off);
-    m = max(m, __shfl_xor_sync(0xffffffffu, m, off));
+    m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, off));
   }
 }
+template <bool WARP_ROW>
+__device__ __forceinline__ void reduce_row(float& s, float2* red) {
+  float none = 0.0f;
+  reduce_row<WARP_ROW>(s, none, red);
+}
 
-__device__ __forceinline__ float silu_mul(float g, float u) { return (g * (1.0f / (1.0f + expf(-g)))) * u; }
+// (the reciprocal is good to one unit in the last place: within the bound of the product's other roundings)
+__device__ __forceinline__ float silu_mul(float g, float u) { return (g * quant::approx_rcp(1.0f + expf(-g))) * u; }
 
-// q[j] = rint(v[j] / s): the product with 1 / s gives the same integer unless it comes near a half-integer (quantize.cuh).
-template <bool VEC>
-__device__ __forceinline__ void store_q(int8_t* p, int step, int left, const float (&v)[8], float s, float inv, bool finite) {
+// q[j] = rint(v[j] / s), inv = 1 / s.  Adding 1.5 * 2^23 to the exact product rounds it to an integer.  EXACT: bit for bit the quotient's, for which octets
+// with a product near a half-integer are divided (quantize.cuh).  finite = false: zeros.
+template <bool ALIGNED, bool EXACT>
+__device__ __forceinline__ void store_q(int8_t* row, int i, int n, const float (&v)[8], float s, float inv, bool finite) {
   uint32_t bits[8];
+  bool sure = true;
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    const float t = v[j] * inv;
-    float r = t + quant::ROUND_MAGIC;
-    if (fabsf(t - (r - quant::ROUND_MAGIC)) > quant::round_limit<8>()) r = rintf(__fdiv_rn(v[j], s)) + quant::ROUND_MAGIC;
-    bits[j] = finite ? __float_as_uint(r) : 0u;
+    const float r = fmaf(v[j], inv, quant::ROUND_MAGIC);
+    if (EXACT) sure = sure && fabsf(fmaf(v[j], inv, quant::ROUND_MAGIC - r)) <= quant::round_limit<8>();
+    bits[j] = __float_as_uint(r);
   }
-  if (VEC) {
-    const uint2 o = quant::pack_octet<8>(bits);
+  if (EXACT && !sure) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) bits[j] = __float_as_uint(rintf(__fdiv_rn(v[j], s)) + quant::ROUND_MAGIC);
+  }
+  uint2 o = quant::pack_octet<8>(bits);
+  if (!finite) o = make_uint2(0u, 0u);
+  int8_t* p = row + i;
+  if (ALIGNED || (i >= 0 && i + 8 <= n && (reinterpret_cast<uintptr_t>(p) & 7) == 0)) {
     *reinterpret_cast<uint2*>(p) = o;
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j * step < left) p[j * step] = static_cast<int8_t>(bits[j]);
+      if (i + j >= 0 && i + j < n) p[j] = static_cast<int8_t>((j < 4 ? o.x : o.y) >> (8 * (j & 3)));
   }
 }
 
-template <typename T, int OP, bool QUANT, bool VEC, int E, bool WARP_ROW, bool WHOLE>
-__global__ void __launch_bounds__(WARP_ROW ? 128 : WHOLE ? 1024 : 512) rows_kernel(const Args p) {
+// E octets a thread; WARP_ROW: four rows a block, a warp each; WHOLE: a row fits into the registers of its threads.
+template <typename T, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
+__global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p) {
+  using Rw = Raw<T, ALIGNED>;
   __shared__ float2 red[2][32];
   griddep_launch_dependents();
   griddep_wait();
-  const long long row = WARP_ROW ? static_cast<long long>(blockIdx.x) * 4 + (threadIdx.x >> 5) : blockIdx.x;
+  const long long row = WARP_ROW ? blockIdx.x * 4ll + (threadIdx.x >> 5) : blockIdx.x;
   if (WARP_ROW && row >= p.n_rows) return;
-  const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x, T_ROW = WARP_ROW ? 32 : blockDim.x;
-  const int step = VEC ? 1 : T_ROW, per_octet = 8 * T_ROW, per_chunk = E * per_octet;
-  const int i0 = VEC ? t * 8 : t;                    // this thread's first value in an octet group
+  const int n = p.n;
+  const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x, per_octet = 8 * (WARP_ROW ? 32 : blockDim.x), per_chunk = E * per_octet;
   const T* a = static_cast<const T*>(p.a) + row * p.lda;
   const T* b = static_cast<const T*>(p.b) + row * p.ldb;
-  const T* gate = static_cast<const T*>(p.gate);
-  if (OP == RESIDUAL && gate) gate += row / p.rows_per_gate * p.n;
   const T* weight = static_cast<const T*>(p.weight);
   const T* post = static_cast<const T*>(p.post_weight);
-  T* hidden = static_cast<T*>(p.hidden_out) + row * p.n;
-  const bool normed = OP == RESIDUAL || (OP == ROWS && weight);
+  const T* gate = static_cast<const T*>(p.gate);
+  if (OP == RESIDUAL && gate) gate += row / p.rows_per_gate * n;
+  T* hidden = static_cast<T*>(p.hidden_out) + row * n;
+  // the first octet begins where the row that is written lies on 16 bytes
+  int i0 = t * 8;
+  if (!ALIGNED && OP == RESIDUAL) i0 -= static_cast<int>((reinterpret_cast<uintptr_t>(hidden) & 15) / sizeof(T));
+  constexpr bool NORMED = OP == RESIDUAL || OP == NORM_ROWS;
+  const auto inside = [&](int i) { return ALIGNED ? i < n : i < n && i + 8 > 0; };
+  const auto factors = [&](const T* src, int i, float(&f)[8]) {
+    Rw w;
+    w.load(src, i, n);
+    w.octet(src, i, n).get(f);
+  };
 
-  Octet<T, VEC> x[E], y[E];                          // RESIDUAL: hidden, delta
-  const auto fetch = [&](Octet<T, VEC>(&o)[E], const T* src, int c0) {
+  Octet<T> x[E], y[E];                               // RESIDUAL: hidden, delta
+  // all loads of a chunk on their way, then the values
+  const auto fetch = [&](const T* src_x, const T* src_y, int c0) {
+    Rw rx[E], ry[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = c0 + e * per_octet + i0;
-      if (i < p.n) o[e].load(src + i, step, p.n - i);
-      else o[e].zero();
+      const int i = i0 + c0 + e * per_octet;
+      if (inside(i)) {
+        if (src_x) rx[e].load(src_x, i, n);
+        if (src_y) ry[e].load(src_y, i, n);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int i = i0 + c0 + e * per_octet;
+      if (inside(i)) {
+        if (src_x) x[e] = rx[e].octet(src_x, i, n);
+        if (src_y) y[e] = ry[e].octet(src_y, i, n);
+      }
     }
   };
-  if (WHOLE) {
-    fetch(x, a, 0);
-    if (OP != ROWS) fetch(y, b, 0);
-  }
+  if (WHOLE) fetch(a, OP == RESIDUAL || OP == SILU_MUL ? b : nullptr, 0);
 
   float rd = 1.0f;                                   // RESIDUAL: 1 / rms of delta
   if (OP == RESIDUAL && post) {
     float ss = 0.0f;
-    uint32_t none = 0u;
-    for (int c0 = 0; c0 < (WHOLE ? 1 : p.n); c0 += per_chunk) {
-      if (!WHOLE) fetch(y, b, c0);
+    for (int c0 = 0; c0 < (WHOLE ? 1 : n + 8); c0 += per_chunk) {
+      if (!WHOLE) fetch(nullptr, b, c0);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
+        if (!inside(i0 + c0 + e * per_octet)) continue;
         float v[8];
         y[e].get(v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
       }
     }
-    reduce_row<WARP_ROW>(ss, none, red[0]);
-    rd = rsqrtf(ss / static_cast<float>(p.n) + p.eps);
+    reduce_row<WARP_ROW>(ss, red[0]);
+    rd = rsqrtf(ss / static_cast<float>(n) + p.eps);
   }
 
-  float ss = 0.0f;
-  uint32_t amax = 0u;
-  const auto magnitude = [&](float v) { amax = max(amax, __float_as_uint(fabsf(v))); };
-  for (int c0 = 0; c0 < (WHOLE ? 1 : p.n); c0 += per_chunk) {
-    if (!WHOLE) {
-      fetch(x, a, c0);
-      if (OP != ROWS) fetch(y, b, c0);
-    }
+  float ss = 0.0f, amax = 0.0f;
+  float value[OP == SILU_MUL ? E : 1][8];            // SILU_MUL: what is quantised
+  for (int c0 = 0; c0 < (WHOLE ? 1 : n + 8); c0 += per_chunk) {
+    if (!WHOLE) fetch(a, OP == RESIDUAL || OP == SILU_MUL ? b : nullptr, c0);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = c0 + e * per_octet + i0;
-      if (i >= p.n) continue;
+      const int i = i0 + c0 + e * per_octet;
+      if (!inside(i)) continue;
       float v[8], u[8];
       x[e].get(v);
-      if (OP == SILU_MUL) {
+      if constexpr (OP == SILU_MUL) {
         y[e].get(u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) magnitude(silu_mul(v[j], u[j]));
+        for (int j = 0; j < 8; ++j) {
+          value[e][j] = silu_mul(v[j], u[j]);
+          amax = max_nan(amax, fabsf(value[e][j]));
+        }
         continue;
       }
       if (OP == RESIDUAL) {
-        y[e].get(u);
-        Octet<T, VEC> o;
         float f[8];
+        y[e].get(u);
         if (post) {
-          o.load(post + i, step, p.n - i);
-          o.get(f);
+          factors(post, i, f);
 #pragma unroll
           for (int j = 0; j < 8; ++j) u[j] = u[j] * rd * f[j];
         }
         if (gate) {
-          o.load(gate + i, step, p.n - i);
-          o.get(f);
+          factors(gate, i, f);
 #pragma unroll
           for (int j = 0; j < 8; ++j) u[j] *= f[j];
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = fmaf(p.scale, u[j], v[j]);
         x[e].set(v);                                 // the value that is stored, which the norm reads
-        x[e].store(hidden + i, step, p.n - i);
+        x[e].template store<ALIGNED>(hidden, i, n);
         x[e].get(v);
       }
-      if (normed) {
+      if (NORMED) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
         if (QUANT) {
-          Octet<T, VEC> o;
-          o.load(weight + i, step, p.n - i);
-          o.get(u);
+          factors(weight, i, u);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) magnitude(v[j] * u[j]);
+          for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j] * u[j]));
         }
-      } else if (QUANT) {
+      } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) magnitude(v[j]);
+        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
       }
     }
   }
   if (!QUANT && !weight) return;                     // RESIDUAL without a norm after it
   reduce_row<WARP_ROW>(ss, amax, red[1]);
-  const float rr = normed ? rsqrtf(ss / static_cast<float>(p.n) + p.eps) : 1.0f;
-  const bool finite = amax < 0x7F800000u;
+  const float rr = NORMED ? rsqrtf(ss / static_cast<float>(n) + p.eps) : 1.0f;
+  const bool finite = amax < __uint_as_float(0x7F800000u);       // (false for NaN)
   // the row's scale, without the factor rr
-  const float s = amax == 0u ? 1.0f : fmaxf(__fdiv_rn(__uint_as_float(amax), 127.0f), 1.17549435e-38f);
+  const float s = amax == 0.0f ? 1.0f : fmaxf(__fdiv_rn(amax, 127.0f), 1.17549435e-38f);
   const float inv = __fdiv_rn(1.0f, s);
-  if (QUANT && t == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : amax == 0u ? 1.0f : normed ? s * rr : s;
+  if (QUANT && t == 0) p.scales[row] = !finite ? __uint_as_float(0x7FC00000u) : amax == 0.0f ? 1.0f : NORMED ? s * rr : s;
 
-  for (int c0 = 0; c0 < (WHOLE ? 1 : p.n); c0 += per_chunk) {
-    if (!WHOLE) {
-      fetch(x, OP == RESIDUAL ? hidden : a, c0);     // (each thread reads what it has written itself)
-      if (OP == SILU_MUL) fetch(y, b, c0);
-    }
+  for (int c0 = 0; c0 < (WHOLE ? 1 : n + 8); c0 += per_chunk) {
+    if (!WHOLE) fetch(OP == RESIDUAL ? hidden : a, OP == SILU_MUL ? b : nullptr, c0);        // (hidden: each thread reads what it has written itself)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const int i = c0 + e * per_octet + i0;
-      if (i >= p.n) continue;
+      const int i = i0 + c0 + e * per_octet;
+      if (!inside(i)) continue;
       float v[8], u[8];
-      x[e].get(v);
-      if (OP == SILU_MUL) {
-        y[e].get(u);
+      if constexpr (OP == SILU_MUL) {
+        if (!WHOLE) {
+          x[e].get(v);
+          y[e].get(u);
+        }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
-      } else if (normed) {
-        Octet<T, VEC> o;
-        o.load(weight + i, step, p.n - i);
-        o.get(u);
+        for (int j = 0; j < 8; ++j) v[j] = WHOLE ? value[e][j] : silu_mul(v[j], u[j]);
+      } else {
+        x[e].get(v);
+        if (NORMED) {
+          factors(weight, i, u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = QUANT ? v[j] * u[j] : v[j] * rr * u[j];
+          for (int j = 0; j < 8; ++j) v[j] = QUANT ? v[j] * u[j] : v[j] * rr * u[j];
+        }
       }
       if (QUANT) {
-        store_q<VEC>(static_cast<int8_t*>(p.out) + row * p.ldo + i, step, p.n - i, v, s, inv, finite);
+        store_q<ALIGNED, OP == ROWS>(static_cast<int8_t*>(p.out) + row * p.ldo, i, n, v, s, inv, finite);
       } else {
-        Octet<T, VEC> o;
+        Octet<T> o;
         o.set(v);
-        o.store(static_cast<T*>(p.out) + row * p.ldo + i, step, p.n - i);
+        o.template store<ALIGNED>(static_cast<T*>(p.out) + row * p.ldo, i, n);
       }
     }
   }
 }
 
 // ---------------------------------------------------------------------------- host side
-template <typename T, int OP, bool QUANT, bool VEC, int E, bool WARP_ROW, bool WHOLE>
+template <typename T, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
 int launch_form(const Args& p, int threads, cudaStream_t st) {
   const long long blocks = WARP_ROW ? (p.n_rows + 3) / 4 : p.n_rows;
-  if (blocks > 2147483647LL) { set_error("too many rows"); return LCQ_ERR_UNSUPPORTED; }
+  if (blocks > 2147483647LL) { set_error("more than 2^31 rows"); return LCQ_ERR_UNSUPPORTED; }
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
   glue::pdl_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(threads), st);
-  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<T, OP, QUANT, VEC, E, WARP_ROW, WHOLE>, p));
+  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<T, OP, QUANT, ALIGNED, E, WARP_ROW, WHOLE, MAX_THREADS, BLOCKS>, p));
   return LCQ_OK;
 }
-template <typename T, int OP, bool QUANT, bool VEC>
-int launch_vec(const Args& p, cudaStream_t st) {
-  const auto threads = [&](int e) { return ((p.n + 8 * e - 1) / (8 * e) + 31) / 32 * 32; };
-  if (p.n <= 512 && p.n_rows >= 4) return launch_form<T, OP, QUANT, VEC, 2, true, true>(p, 128, st);
-  if (p.n <= 8192) return launch_form<T, OP, QUANT, VEC, 1, false, true>(p, threads(1), st);
-  if (p.n <= 16384) return launch_form<T, OP, QUANT, VEC, 2, false, true>(p, threads(2), st);
-  return launch_form<T, OP, QUANT, VEC, 2, false, false>(p, 512, st);
+// The forms and where each is the faster (us, B200; n values a row, E octets a thread).
+//   a warp a row, four rows a block   n <= 512 (20,000 x 512 quantised: 8.1, 21.3 with a block a row, whose launches bound it), and <= 1024 with one operand
+//   E = 1, most threads a row         few rows, where latency counts (1 x 4096: 2.6; E = 2 3.2, E = 4 4.4), and RESIDUAL up to 2048 values or 8 Mi in all
+//   E = 4, most bytes on their way    all other 16-bit rows up to 16,384 (8192 x 8192 RESIDUAL: 87; E = 1 122, E = 2 98, E = 8 101)
+//   E = 2                             float32, and rows off 16 bytes, which hold more registers for each octet (4000 x 5003: 48; E = 1 59, E = 4 56)
+//   E = 8                             16-bit rows up to 32,768 (1000 x 28,672 SILU_MUL: 45; in chunks 58)
+template <typename T, int OP, bool QUANT, bool ALIGNED>
+int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
+  constexpr bool HALF = sizeof(T) == 2, ONE = OP == ROWS || OP == NORM_ROWS;
+  const int span = p.n + (ALIGNED ? 0 : 7);          // (an octet may begin up to seven values before the row)
+  const auto threads = [&](int e) { return ((span + 8 * e - 1) / (8 * e) + 31) / 32 * 32; };
+  const bool few = p.n_rows <= 2ll * sm_count;
+  if (span <= 512 && p.n_rows >= 4) return launch_form<T, OP, QUANT, ALIGNED, 2, true, true, 128, 8>(p, 128, st);
+  if constexpr (ONE) {
+    if (span <= 1024 && !few) return launch_form<T, OP, QUANT, ALIGNED, 4, true, true, 128, 4>(p, 128, st);
+  }
+  if (span <= 8192 && (few || (HALF && ALIGNED && OP == RESIDUAL && (p.n <= 2048 || p.n_rows * p.n <= (8ll << 20)))))
+    return launch_form<T, OP, QUANT, ALIGNED, 1, false, true, 1024, 2>(p, threads(1), st);
+  if constexpr (!HALF || !ALIGNED) {
+    if (span <= 8192) return launch_form<T, OP, QUANT, ALIGNED, 2, false, true, 512, 2>(p, threads(2), st);
+    if (span <= 16384) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 512, 1>(p, threads(4), st);
+  } else {
+    if (span <= 16384) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 512, ONE ? 3 : 2>(p, threads(4), st);
+  }
+  if constexpr (HALF) {
+    if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 8, false, true, 512, ONE ? 2 : 1>(p, threads(8), st);
+  }
+  return launch_form<T, OP, QUANT, ALIGNED, 2, false, false, 512, 2>(p, 512, st);
 }
-// Octets of consecutive values where every row of every operand starts on 16 bytes (of q: on 8).
+
+// Octets as they lie where every row of every operand starts on 16 bytes (of q: on 8) and holds whole ones.
 template <typename T, int OP, bool QUANT>
-int launch(const Args& p, cudaStream_t st) {
+int launch(const Args& p, int sm_count, cudaStream_t st) {
   const auto rows_on_16 = [&](const void* q, long long ld) { return aligned(q, 16) && (ld * sizeof(T)) % 16 == 0; };
-  const bool vec = p.n % 8 == 0 && rows_on_16(p.a, p.lda) && rows_on_16(p.b, p.ldb) && aligned(p.weight, 16) && aligned(p.post_weight, 16) &&
-                   aligned(p.gate, 16) && aligned(p.hidden_out, 16) &&
-                   (QUANT ? aligned(p.out, 8) && p.ldo % 8 == 0 : rows_on_16(p.out, p.ldo));
-  return vec ? launch_vec<T, OP, QUANT, true>(p, st) : launch_vec<T, OP, QUANT, false>(p, st);
+  const bool on_16 = p.n % 8 == 0 && rows_on_16(p.a, p.lda) && rows_on_16(p.b, p.ldb) && aligned(p.weight, 16) && aligned(p.post_weight, 16) &&
+                     aligned(p.gate, 16) && aligned(p.hidden_out, 16) &&
+                     (QUANT ? aligned(p.out, 8) && p.ldo % 8 == 0 : rows_on_16(p.out, p.ldo));
+  return on_16 ? launch_aligned<T, OP, QUANT, true>(p, sm_count, st) : launch_aligned<T, OP, QUANT, false>(p, sm_count, st);
 }
 
 }  // namespace rows
