@@ -88,11 +88,15 @@ class DecodeStack:
     norm, and a greedy argmax of the logits on the device -- a real dependency chain on one hidden
     state.  In fp16 the whole step is one kernel where that covers the shape and is faster, else 8 launches per layer.
     Since o reads a prepared buffer and not attention output, that kernel computes it two layers
-    ahead: two dependent phases a layer, where a model with attention has four."""
+    ahead: two dependent phases a layer, where a model with attention has four.
+    `int8=True` (with glue) runs the same chain in int8: weights with one scale for each output channel, every linear on int8
+    tokens with a scale each (int8_matmul), and the norms between them as one launch that also quantises (residual_norms): 7 launches
+    per layer.  `post_norms=True` (with int8) normalises the output of each block before it is added, with weights of its own, and
+    `residual_scale` multiplies it: the layer form residual_norms is for."""
 
     def __init__(self, layers: int = 30, hidden: int = 576, inter: int = 1536, q_heads: int = 9, kv_heads: int = 3,
                  head_dim: int = 64, vocab: int = 49152, fused: bool = False, device="cuda", seed: int = 0,
-                 dtype=torch.float16, glue: bool = False):
+                 dtype=torch.float16, glue: bool = False, int8: bool = False, post_norms: bool = False, residual_scale: float = 1.0):
         g = torch.Generator(device=device).manual_seed(seed)
 
         def make(n, k):
@@ -102,7 +106,12 @@ class DecodeStack:
         qd, kvd = q_heads * head_dim, kv_heads * head_dim
         if glue and not fused:
             raise ValueError("glue=True runs the fused layer form")
+        if int8 and not glue:
+            raise ValueError("int8=True runs the form with glue")
+        if not int8 and (post_norms or residual_scale != 1.0):
+            raise ValueError("post_norms and residual_scale are of the int8 form")
         self.glue = glue
+        self.int8 = int8
         self.ops = []                                  # with glue: the step as a list of zero-argument launches
         self._desc = None                              # with glue, where one kernel covers the shape: its description
         self.calls: List[Tuple[QuantLinear, torch.Tensor, torch.Tensor]] = []   # (linear, x, out)
@@ -112,7 +121,10 @@ class DecodeStack:
 
         def add(lin, x):
             self.calls.append((lin, x, torch.empty(1, lin.out_features, dtype=dtype, device=device)))
-        if glue:
+        if int8:
+            self._int8_chain(layers, hidden, inter, qd, qd + 2 * kvd, vocab, dtype, device, g, x_q, post_norms, residual_scale)
+            layers = 0                                 # the plain construction below adds nothing more
+        elif glue:
             from . import decode_ops as D
             self.table = (torch.randn(vocab, hidden, device=device, generator=g) * 0.02).to(dtype)
             self.token = torch.zeros(1, dtype=torch.int32, device=device)
@@ -179,10 +191,54 @@ class DecodeStack:
         # one scratch buffer for the whole stack (calls are stream-ordered), allocated up front so
         # that nothing is allocated while a CUDA graph is being captured
         kind = _TORCH_TO_KIND[dtype]
-        need = max(matmul_workspace_bytes(1, c[0].out_features, c[0].in_features, 32, 4, kind, "f16", kind)
-                   for c in self.calls)
+        need = 0 if int8 else max(matmul_workspace_bytes(1, c[0].out_features, c[0].in_features, 32, 4, kind, "f16", kind)
+                                  for c in self.calls)
         self.workspace = torch.zeros(max(need, 256), dtype=torch.uint8, device=device)
         self._graph = None
+
+    def _int8_chain(self, layers, hidden, inter, qd, qkv, vocab, dtype, device, g, x_q, post_norms, scale):
+        """The step in int8.  `hidden` is the residual stream; the tokens between the launches live in fixed buffers."""
+        from . import decode_ops as D
+        from .int8_ops import Int8Linear, _empty_tokens, quantize_tokens, residual_norms, silu_mul_tokens
+
+        def layer(n, k):
+            w = torch.randint(-127, 128, (n, k), dtype=torch.int8, device=device, generator=g)
+            return Int8Linear(w, torch.rand(n, device=device, generator=g) * (0.02 / k ** 0.5))
+
+        def norm():
+            return (1 + 0.1 * torch.randn(hidden, device=device, generator=g)).to(dtype)
+
+        def empty(n):
+            return torch.empty(1, n, dtype=dtype, device=device)
+        self.table = (torch.randn(vocab, hidden, device=device, generator=g) * 0.02).to(dtype)
+        self.token, self.next_token = (torch.zeros(1, dtype=torch.int32, device=device) for _ in range(2))
+        self.hidden = torch.zeros(1, hidden, dtype=dtype, device=device)
+        self.normed, self.mlp = _empty_tokens((1, hidden), device), _empty_tokens((1, inter), device)
+        self.attention = quantize_tokens(x_q)          # attention is not part of this path: o reads prepared tokens
+        first = norm()
+        self.norms = [first]
+
+        def product(lin, tokens):
+            out = empty(lin.out_features)
+            self.calls.append((lin, tokens, out))
+            self.ops.append(lambda: lin(tokens, out=out))
+            return out
+
+        def to_next_block(delta):                      # the norm after the block (if any), the residual, the norm before the next
+            post, weight = norm() if post_norms else None, norm()
+            self.norms += [weight] if post is None else [post, weight]
+            self.ops.append(lambda: residual_norms(self.hidden, delta, weight, 1e-5, post_weight=post, scale=scale, out=self.normed,
+                                                   quantized=True))
+        self.ops.append(lambda: D.embed_lookup(self.token, self.table, self.hidden, 1, hidden))
+        self.ops.append(lambda: quantize_tokens(self.hidden, first, 1e-5, out=self.normed))
+        for _ in range(layers):
+            product(layer(qkv, hidden), self.normed)
+            to_next_block(product(layer(hidden, qd), self.attention))
+            gu = product(layer(2 * inter, hidden), self.normed)
+            self.ops.append(lambda gu=gu: silu_mul_tokens(gu[:, :inter], gu[:, inter:], out=self.mlp))
+            to_next_block(product(layer(hidden, inter), self.mlp))
+        self.logits = product(layer(vocab, hidden), self.normed)
+        self.ops.append(lambda: D.argmax(self.logits, out=self.next_token))
 
     def _one_kernel(self, x_q, layers, hidden, inter, qd, qkv, vocab):
         """Describe the step to the kernel that runs all of it, if it covers the shape (fp16 only) and is faster."""

@@ -630,3 +630,62 @@ def test_rows_on_another_stream():
     side.synchronize()
     b = L.quantize_tokens(x, w)
     assert torch.equal(a.q, b.q) and torch.equal(n, L.residual_norms(x.clone(), x, w)) and torch.equal(s.q, L.silu_mul_tokens(x, x).q)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("post_norms,scale", [(False, 1.0), (True, 0.5)])
+def test_decode_stack_in_int8(kind, post_norms, scale):
+    """Every launch of two layers against 64 bits on what the launches before it left, and the same step from a graph."""
+    st = L.DecodeStack(layers=2, hidden=200, inter=333, q_heads=3, kv_heads=1, head_dim=40, vocab=1000, fused=True, glue=True, int8=True, dtype=kind,
+                       post_norms=post_norms, residual_scale=scale, seed=4)
+    assert st.launches_per_step == len(st.ops) == 2 + 7 * 2 + 2
+    st.token.fill_(77)
+    for t in (st.normed, st.mlp):
+        t.q.zero_()
+    ops, norms, calls = iter(st.ops), iter(st.norms), iter(st.calls)
+
+    def linear():
+        lin, tokens, out = next(calls)
+        next(ops)()
+        ref = tokens.q.double() @ lin.w.double().t() * tokens.scales.double()[:, None] * lin.scales.double()
+        check_product(out, ref, kind)
+        return out
+
+    def block_end(delta):
+        before = st.hidden.double()
+        next(ops)()
+        y = rms(delta.double(), next(norms)) if post_norms else delta.double()
+        ref = before + scale * y
+        assert bool(((st.hidden.double() - ref).abs() <= (HALF_STEP[kind] + 2 * REL) * (ref.abs() + before.abs()) + 2.0 ** -25).all())
+        check_tokens(st.normed, rms(st.hidden.double(), next(norms)))
+    next(ops)()
+    assert torch.equal(st.hidden[0], st.table[77])
+    next(ops)()
+    check_tokens(st.normed, rms(st.hidden.double(), next(norms)))
+    for _ in range(2):
+        linear()
+        block_end(linear())
+        gu = linear()
+        next(ops)()
+        a, b = gu[:, :333].double(), gu[:, 333:].double()
+        check_tokens(st.mlp, a * torch.sigmoid(a) * b)
+        block_end(linear())
+    logits = linear()
+    next(ops)()
+    assert int(st.next_token) == int(logits.float().argmax()) and not list(ops) and not list(norms)
+    want, token = logits.clone(), int(st.next_token)
+    st.capture()
+    logits.zero_()
+    st.next_token.zero_()
+    st.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(st.logits, want) and int(st.next_token) == token
+    status_ok()
+
+
+def test_decode_stack_says_what_int8_needs():
+    with pytest.raises(ValueError, match="glue"):
+        L.DecodeStack(layers=1, fused=True, int8=True, device="cpu")
+    with pytest.raises(ValueError, match="int8 form"):
+        L.DecodeStack(layers=1, fused=True, glue=True, post_norms=True, device="cpu")
