@@ -678,6 +678,10 @@ inline Tiling choose_tiling(int M, int N, int K, int sm_count, const ClusterFit&
       }
     }
   }
+  // No more stages than a team has use for (and the cluster's exchange needs): a small call then leaves room on the SM for the next kernel's start.
+  const long long stages = best.split > 1 ? (nst + best.split - 1) / best.split : (static_cast<long long>(best.n_tiles) + best.teams - 1) / best.teams * nst;
+  const int exchange = best.split > 1 ? ((M < best.bm ? M : best.bm) + best.split - 1) / best.split * best.split * BN * 4 : 0;
+  while (best.depth > 2 && best.depth > stages && (best.depth - 1) * stage_bytes(best.bm, best.cg) >= exchange) --best.depth;
   return best;
 }
 

@@ -761,7 +761,7 @@ int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void
   o.w = w; o.ldw = ldw;
   o.w_scales = w_scales; o.w_scale_dtype = w_scale_dtype;
   o.out = out; o.ldo = N; o.out_dtype = out_dtype;
-  if (int8_gemv::takes(M, N, K, int8_gemm::mappable(x, ldx) && int8_gemm::mappable(w, ldw))) return int8_gemv::launch(o, M, N, K, static_cast<cudaStream_t>(stream));
+  if (int8_gemv::takes(M, N, K, int8_gemm::mappable(x, ldx) && int8_gemm::mappable(w, ldw))) return int8_gemv::launch(o, M, N, K, di.sm_count, static_cast<cudaStream_t>(stream));
   return int8_gemm::launch(o, M, N, K, workspace, workspace_bytes, di.sm_count, device_cluster_fit(di.sm_count), static_cast<cudaStream_t>(stream));
 }
 
