@@ -255,47 +255,58 @@ __device__ __forceinline__ float2 unpack2(uint64_t a) {
   asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
   return r;
 }
-__device__ __forceinline__ void put2(float* p, int stride, float2 v) { p[0] = v.x; p[stride] = v.y; }
-__device__ __forceinline__ void put2(__half* p, int stride, float2 v) {
+__device__ __forceinline__ void put2(float* p, float* q, float2 v) { *p = v.x; *q = v.y; }
+__device__ __forceinline__ void put2(__half* p, __half* q, float2 v) {
   const __half2 h = __floats2half2_rn(v.x, v.y);
-  p[0] = __low2half(h);
-  p[stride] = __high2half(h);
+  *p = __low2half(h);
+  *q = __high2half(h);
 }
-__device__ __forceinline__ void put2(__nv_bfloat16* p, int stride, float2 v) {
+__device__ __forceinline__ void put2(__nv_bfloat16* p, __nv_bfloat16* q, float2 v) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(v.x, v.y);
-  p[0] = __low2bfloat16(h);
-  p[stride] = __high2bfloat16(h);
+  *p = __low2bfloat16(h);
+  *q = __high2bfloat16(h);
 }
 
+// Where rows of out do not start on 16 bytes, a row's 128 channels lie rotated in shared memory, by the place of its first one in its 16 bytes of global
+// memory: so that sixteen bytes are sixteen bytes on both sides.  EACH values in 16 bytes.
+struct Rotation {
+  int first, step;                             // of the chunk's first token; from token to token
+  __device__ __forceinline__ int of(int row, int each) const { return (first + row * step) & (each - 1); }
+};
 // A chunk into shared memory, [token][128 channels]: from there 256 (512) consecutive bytes of a token go out together.  (Stored from registers, 64 or 128
 // bytes a warp, a 1024 x 16384 output took 56 us in 16 bits and 32 us in float32, whatever K.)
-template <typename OT, int C>
-__device__ __forceinline__ void stage_chunk(const uint32_t (&v)[C], OT* mine, const float* xs, uint64_t ws2) {
+template <typename OT, int C, bool ROTATED>
+__device__ __forceinline__ void stage_chunk(const uint32_t (&v)[C], OT* buf, int r, Rotation rot, const float* xs, uint64_t ws2) {
+  constexpr int EACH = 16 / static_cast<int>(sizeof(OT));
+  const auto at = [&](int i) { return buf + i * BN + (ROTATED ? (r + rot.of(i, EACH)) & (BN - 1) : r); };
 #pragma unroll
   for (int i = 0; i < C; i += 4) {
     const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(xs + i);
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
       const uint64_t sum = pack2(static_cast<float>(static_cast<int>(v[i + j])), static_cast<float>(static_cast<int>(v[i + j + 1])));
-      put2(mine + (i + j) * BN, BN, unpack2(mul2(mul2(sum, j == 0 ? s.x : s.y), ws2)));
+      put2(at(i + j), at(i + j + 1), unpack2(mul2(mul2(sum, j == 0 ? s.x : s.y), ws2)));
     }
   }
 }
-// The chunk's rows from shared memory, where rows of out do not start on 16 bytes; a group's four warps.
-template <typename OT>
-__device__ __forceinline__ void store_rows(const OT* buf, OT* out, long long ldo, int channels, int columns, int warp, int lane) {
-  for (int row = warp; row < columns; row += 4) {
+// A chunk's rotated rows from shared memory to global, by a group's 128 threads: 16 bytes a thread, but for those that hold a row's first and last channels.
+template <typename OT, int C>
+__device__ __forceinline__ void store_rotated(const OT* buf, OT* out, long long ldo, Rotation rot, int channels, int columns, int t) {
+  constexpr int EACH = 16 / static_cast<int>(sizeof(OT)), PIECES = BN / EACH;
+#pragma unroll
+  for (int i = 0; i < C * PIECES / 128; ++i) {
+    const int row = (i * 128 + t) / PIECES, piece = t % PIECES;
+    if (row >= columns) break;
+    const int shift = rot.of(row, EACH), c0 = piece * EACH - shift;
     OT* o = out + row * ldo;
-    const OT* src = buf + row * BN;
-    if constexpr (sizeof(OT) == 4) {
-      for (int j = lane; j < channels; j += 32) o[j] = src[j];
-    } else {                                     // pairs on 4 bytes, wherever the row starts
-      const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-      const int head = (reinterpret_cast<uintptr_t>(o) & 2) ? 1 : 0;
-      if (lane == 0 && head && channels > 0) o[0] = src[0];
-      for (int j = head + 2 * lane; j < channels; j += 64) {
-        if (j + 1 < channels) *reinterpret_cast<uint32_t*>(o + j) = h[j] | static_cast<uint32_t>(h[j + 1]) << 16;
-        else o[j] = src[j];
+    const OT* src = buf + row * BN + piece * EACH;
+    if (c0 >= 0 && c0 + EACH <= channels) {
+      *reinterpret_cast<uint4*>(o + c0) = *reinterpret_cast<const uint4*>(src);
+    } else {
+#pragma unroll
+      for (int e = 0; e < EACH; ++e) {
+        const int c = (c0 + e) & (BN - 1);
+        if (c < channels) o[c] = src[e];
       }
     }
   }
@@ -466,8 +477,8 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         const int columns = rows - c0 < C ? rows - c0 : C;
         if (stage_out) {
           OT* buf = reinterpret_cast<OT*>(buffers + buffer * OUT_BUFFER);
-          stage_chunk<OT, C>(v, buf + r, xs_tile + c0, pack2(ws, ws));
           if (p.vec) {
+            stage_chunk<OT, C, false>(v, buf, r, {0, 0}, xs_tile + c0, pack2(ws, ws));
             fence_async_smem();                // the copy reads through the async proxy
             if (in_group == 0 && lane == 0) tma_stores_read();        // the copy before this one has left the other buffer, which comes next
             named_bar_sync(BAR_GROUP + group, 128);
@@ -475,8 +486,11 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
               for (int h = 0; h < columns; h += OUT_BOX) tma_store_2d(&tmap_out, buf + h * BN, n0, m0 + c0 + h);
             }
           } else {
+            OT* o = out + c0 * p.ldo;
+            const Rotation rot = {static_cast<int>(reinterpret_cast<uintptr_t>(o) / sizeof(OT) & 7), static_cast<int>(p.ldo & 7)};
+            stage_chunk<OT, C, true>(v, buf, r, rot, xs_tile + c0, pack2(ws, ws));
             named_bar_sync(BAR_GROUP + group, 128);
-            store_rows<OT>(buf, out + c0 * p.ldo, p.ldo, p.N - n0 < BN ? p.N - n0 : BN, columns, in_group, lane);
+            store_rotated<OT, C>(buf, o, p.ldo, rot, p.N - n0 < BN ? p.N - n0 : BN, columns, r);
           }
           buffer ^= 1;
         } else {
