@@ -240,21 +240,6 @@ __device__ __forceinline__ void store_direct(const uint32_t (&v)[C], OT* out, lo
   }
 }
 
-__device__ __forceinline__ uint64_t pack2(float a, float b) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
-  return r;
-}
-__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-__device__ __forceinline__ float2 unpack2(uint64_t a) {
-  float2 r;
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a));
-  return r;
-}
 __device__ __forceinline__ void put2(float* p, float* q, float2 v) { *p = v.x; *q = v.y; }
 __device__ __forceinline__ void put2(__half* p, __half* q, float2 v) {
   const __half2 h = __floats2half2_rn(v.x, v.y);
@@ -284,8 +269,8 @@ __device__ __forceinline__ void stage_chunk(const uint32_t (&v)[C], OT* buf, int
     const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(xs + i);
 #pragma unroll
     for (int j = 0; j < 4; j += 2) {
-      const uint64_t sum = pack2(static_cast<float>(static_cast<int>(v[i + j])), static_cast<float>(static_cast<int>(v[i + j + 1])));
-      put2(at(i + j), at(i + j + 1), unpack2(mul2(mul2(sum, j == 0 ? s.x : s.y), ws2)));
+      const uint64_t sum = pack_pair(static_cast<float>(static_cast<int>(v[i + j])), static_cast<float>(static_cast<int>(v[i + j + 1])));
+      put2(at(i + j), at(i + j + 1), unpack_pair(mul_pair(mul_pair(sum, j == 0 ? s.x : s.y), ws2)));
     }
   }
 }
@@ -478,7 +463,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
         if (stage_out) {
           OT* buf = reinterpret_cast<OT*>(buffers + buffer * OUT_BUFFER);
           if (p.vec) {
-            stage_chunk<OT, C, false>(v, buf, r, {0, 0}, xs_tile + c0, pack2(ws, ws));
+            stage_chunk<OT, C, false>(v, buf, r, {0, 0}, xs_tile + c0, pack_pair(ws, ws));
             fence_async_smem();                // the copy reads through the async proxy
             if (in_group == 0 && lane == 0) tma_stores_read();        // the copy before this one has left the other buffer, which comes next
             named_bar_sync(BAR_GROUP + group, 128);
@@ -488,7 +473,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
           } else {
             OT* o = out + c0 * p.ldo;
             const Rotation rot = {static_cast<int>(reinterpret_cast<uintptr_t>(o) / sizeof(OT) & 7), static_cast<int>(p.ldo & 7)};
-            stage_chunk<OT, C, true>(v, buf, r, rot, xs_tile + c0, pack2(ws, ws));
+            stage_chunk<OT, C, true>(v, buf, r, rot, xs_tile + c0, pack_pair(ws, ws));
             named_bar_sync(BAR_GROUP + group, 128);
             store_rotated<OT, C>(buf, o, p.ldo, rot, p.N - n0 < BN ? p.N - n0 : BN, columns, r);
           }
@@ -594,28 +579,35 @@ struct Piece {
     return make_uint4(r[0], r[1], r[2], r[3]);
   }
 };
-// Rows of K bytes, ld apart, into rows of `per_row` pieces of 16 bytes (the last one filled up with zeros).  total < 2^31 pieces.
-__global__ void __launch_bounds__(256) align_rows_kernel(const uint8_t* src, long long ld, uint4* dst, int K, int per_row, Divisor by_per_row, int total) {
+// Rows of K bytes, ld apart, into rows of `per_row` pieces of 16 bytes (the last one filled up with zeros): of two operands, one after the other.
+struct AlignJob {
+  const uint8_t* src;
+  long long ld;
+  uint4* dst;
+  int pieces;                // all in all
+};
+__global__ void __launch_bounds__(256) align_rows_kernel(const AlignJob first, const AlignJob second, int K, int per_row, Divisor by_per_row) {
   griddep_launch_dependents();
   griddep_wait();
   constexpr int EACH = 4;
-  const int stride = static_cast<int>(gridDim.x) * 256;
-  for (long long i0 = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i0 < total; i0 += EACH * stride) {
+  const long long stride = gridDim.x * 256ll, total = static_cast<long long>(first.pieces) + second.pieces;
+  for (long long i0 = blockIdx.x * 256ll + threadIdx.x; i0 < total; i0 += EACH * stride) {
     Piece v[EACH];
+    uint4* dst[EACH];
     int valid[EACH];
 #pragma unroll
     for (int j = 0; j < EACH; ++j) {
-      const long long i = i0 + static_cast<long long>(j) * stride;
-      const int at = i < total ? static_cast<int>(i) : 0;
+      const long long i = i0 + j * stride;
+      const AlignJob& job = i < first.pieces ? first : second;
+      const int at = i < total ? static_cast<int>(i < first.pieces ? i : i - first.pieces) : 0;
       const int row = by_per_row.divide(at), k = (at - row * per_row) * 16;
+      dst[j] = job.dst + at;
       valid[j] = i < total ? K - k : 0;
-      v[j].load(src + row * ld + k, valid[j]);
+      v[j].load(job.src + row * job.ld + k, valid[j]);
     }
 #pragma unroll
-    for (int j = 0; j < EACH; ++j) {
-      const long long i = i0 + static_cast<long long>(j) * stride;
-      if (i < total) dst[i] = v[j].get(valid[j]);
-    }
+    for (int j = 0; j < EACH; ++j)
+      if (i0 + j * stride < total) *dst[j] = v[j].get(valid[j]);
   }
 }
 
@@ -807,18 +799,27 @@ inline int launch_tiling(const Tiling& t, const Operands& o, int M, int N, int K
   return LCQ_ERR_BAD_ARG;
 }
 
-inline int launch_align(const void* src, long long ld, void* dst, long long rows, int K, int sm_count, cudaStream_t stream) {
+struct Rows { const void* src; long long ld; void* dst; long long rows; };
+// Copies up to 2^30 pieces of 16 bytes of each of two operands in a launch.
+inline int launch_align(Rows a, Rows b, int K, int sm_count, cudaStream_t stream) {
   const int per_row = (K + 15) / 16;
   const long long most = (1ll << 30) / per_row;
-  for (long long r = 0; r < rows; r += most) {
-    const long long n = rows - r < most ? rows - r : most, total = n * per_row;
-    long long blocks = (total + 1023) / 1024;
+  const auto take = [&](Rows& r) {
+    const long long n = r.rows < most ? r.rows : most;
+    const AlignJob job = {static_cast<const uint8_t*>(r.src), r.ld, static_cast<uint4*>(r.dst), static_cast<int>(n * per_row)};
+    r.src = static_cast<const uint8_t*>(r.src) + n * r.ld;
+    r.dst = static_cast<uint4*>(r.dst) + n * per_row;
+    r.rows -= n;
+    return job;
+  };
+  while (a.rows > 0 || b.rows > 0) {
+    const AlignJob first = take(a), second = take(b);
+    long long blocks = (static_cast<long long>(first.pieces) + second.pieces + 1023) / 1024;
     if (blocks > sm_count * 8ll) blocks = sm_count * 8ll;
     cudaLaunchConfig_t cfg;
     cudaLaunchAttribute attr[1];
     gemm_tc::pdl_launch_config(cfg, attr, static_cast<int>(blocks), 256, 0, stream);
-    LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, align_rows_kernel, static_cast<const uint8_t*>(src) + r * ld, ld, static_cast<uint4*>(dst) + r * per_row, K, per_row,
-                                    make_divisor(per_row), static_cast<int>(total)));
+    LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, align_rows_kernel, first, second, K, per_row, make_divisor(per_row)));
   }
   return LCQ_OK;
 }
@@ -833,9 +834,9 @@ inline int launch(Operands o, int M, int N, int K, void* workspace, size_t ws_by
   }
   uint8_t* scratch = need ? static_cast<uint8_t*>(workspace) + kWorkspaceCounterBytes : nullptr;
   const long long row = (static_cast<long long>(K) + 15) / 16 * 16;
+  const Rows none = {nullptr, 0, nullptr, 0};
+  const Rows x_rows = {o.x, o.ldx, scratch, M};
   if (!x_mappable) {
-    const int rc = launch_align(o.x, o.ldx, scratch, M, K, sm_count, stream);
-    if (rc != LCQ_OK) return rc;
     o.x = scratch;
     o.ldx = row;
   }
@@ -845,9 +846,13 @@ inline int launch(Operands o, int M, int N, int K, void* workspace, size_t ws_by
   const long long ldw = o.ldw;
   for (int n0 = 0; n0 < N; n0 += q.piece) {
     const int n = N - n0 < q.piece ? N - n0 : q.piece;
-    if (!w_mappable) {
-      const int rc = launch_align(w + n0 * ldw, ldw, scratch + q.x_copy, n, K, sm_count, stream);
+    const bool copy_x = !x_mappable && n0 == 0;
+    if (copy_x || !w_mappable) {
+      const Rows w_rows = {w + n0 * ldw, ldw, scratch + q.x_copy, n};
+      const int rc = launch_align(copy_x ? x_rows : none, w_mappable ? none : w_rows, K, sm_count, stream);
       if (rc != LCQ_OK) return rc;
+    }
+    if (!w_mappable) {
       o.w = scratch + q.x_copy;
       o.ldw = row;
     }

@@ -124,6 +124,49 @@ template <typename T> struct Raw<T, false> {
   }
 };
 
+// Eight values at a time.  PAIRS: two an instruction, since instructions bound these rows as much as memory does; one by one where registers are short.
+template <bool PAIRS> __device__ __forceinline__ void mul8(float (&a)[8], const float (&b)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 r = PAIRS ? unpack_pair(mul_pair(pack_pair(a[j], a[j + 1]), pack_pair(b[j], b[j + 1]))) : make_float2(a[j] * b[j], a[j + 1] * b[j + 1]);
+    a[j] = r.x;
+    a[j + 1] = r.y;
+  }
+}
+template <bool PAIRS> __device__ __forceinline__ void scale8(float (&a)[8], float s) {
+  const float t[8] = {s, s, s, s, s, s, s, s};
+  mul8<PAIRS>(a, t);
+}
+template <bool PAIRS> __device__ __forceinline__ void add_scaled8(float (&v)[8], float s, const float (&u)[8]) {      // v += s * u
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) {
+    const float2 r = PAIRS ? unpack_pair(fma_pair(pack_pair(s, s), pack_pair(u[j], u[j + 1]), pack_pair(v[j], v[j + 1])))
+                           : make_float2(fmaf(s, u[j], v[j]), fmaf(s, u[j + 1], v[j + 1]));
+    v[j] = r.x;
+    v[j + 1] = r.y;
+  }
+}
+struct Squares {             // two sums, the same ones either way
+  uint64_t two = 0;
+  float one = 0.0f, other = 0.0f;
+  template <bool PAIRS> __device__ __forceinline__ void add(const float (&v)[8]) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 2) {
+      if (PAIRS) {
+        const uint64_t p = pack_pair(v[j], v[j + 1]);
+        two = fma_pair(p, p, two);
+      } else {
+        one = fmaf(v[j], v[j], one);
+        other = fmaf(v[j + 1], v[j + 1], other);
+      }
+    }
+  }
+  template <bool PAIRS> __device__ __forceinline__ float sum() const {
+    const float2 r = unpack_pair(two);
+    return PAIRS ? r.x + r.y : one + other;
+  }
+};
+
 // The larger magnitude, or NaN where there is one.
 __device__ __forceinline__ float max_nan(float a, float b) {
   float r;
@@ -166,14 +209,20 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return (g * quant:
 template <bool ALIGNED, bool EXACT>
 __device__ __forceinline__ void store_q(int8_t* row, int i, int n, const float (&v)[8], float s, float inv, bool finite) {
   uint32_t bits[8];
-  bool sure = true;
+  float off = 0.0f;                                  // how far the products are from their integers, at most
+  const uint64_t inv2 = pack_pair(inv, inv), magic2 = pack_pair(quant::ROUND_MAGIC, quant::ROUND_MAGIC), minus2 = pack_pair(-1.0f, -1.0f);
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float r = fmaf(v[j], inv, quant::ROUND_MAGIC);
-    if (EXACT) sure = sure && fabsf(fmaf(v[j], inv, quant::ROUND_MAGIC - r)) <= quant::round_limit<8>();
-    bits[j] = __float_as_uint(r);
+  for (int j = 0; j < 8; j += 2) {
+    const uint64_t v2 = pack_pair(v[j], v[j + 1]), r2 = fma_pair(v2, inv2, magic2);
+    const float2 r = unpack_pair(r2);
+    if (EXACT) {
+      const float2 d = unpack_pair(fma_pair(v2, inv2, fma_pair(r2, minus2, magic2)));
+      off = fmaxf(off, fmaxf(fabsf(d.x), fabsf(d.y)));
+    }
+    bits[j] = __float_as_uint(r.x);
+    bits[j + 1] = __float_as_uint(r.y);
   }
-  if (EXACT && !sure) {
+  if (EXACT && off > quant::round_limit<8>()) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) bits[j] = __float_as_uint(rintf(__fdiv_rn(v[j], s)) + quant::ROUND_MAGIC);
   }
@@ -193,6 +242,7 @@ __device__ __forceinline__ void store_q(int8_t* row, int i, int n, const float (
 template <typename T, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
 __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p) {
   using Rw = Raw<T, ALIGNED>;
+  constexpr bool PAIRS = ALIGNED || sizeof(T) == 2;
   __shared__ float2 red[2][32];
   griddep_launch_dependents();
   griddep_wait();
@@ -243,7 +293,7 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
 
   float rd = 1.0f;                                   // RESIDUAL: 1 / rms of delta
   if (OP == RESIDUAL && post) {
-    float ss = 0.0f;
+    Squares squares;
     for (int c0 = 0; c0 < (WHOLE ? 1 : n + 8); c0 += per_chunk) {
       if (!WHOLE) fetch(nullptr, b, c0);
 #pragma unroll
@@ -251,16 +301,18 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
         if (!inside(i0 + c0 + e * per_octet)) continue;
         float v[8];
         y[e].get(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        squares.template add<PAIRS>(v);
       }
     }
+    float ss = squares.template sum<PAIRS>();
     reduce_row<WARP_ROW>(ss, red[0]);
     rd = rsqrtf(ss / static_cast<float>(n) + p.eps);
   }
 
-  float ss = 0.0f, amax = 0.0f;
-  float value[OP == SILU_MUL ? E : 1][8];            // SILU_MUL: what is quantised
+  Squares squares;
+  float amax = 0.0f;
+  constexpr bool KEEP = WHOLE && QUANT && (OP == SILU_MUL || (OP != ROWS && PAIRS && E <= 4));
+  float value[KEEP ? E : 1][8];                      // what is quantised (of NORMED rows without the factor rr)
   for (int c0 = 0; c0 < (WHOLE ? 1 : n + 8); c0 += per_chunk) {
     if (!WHOLE) fetch(a, OP == RESIDUAL || OP == SILU_MUL ? b : nullptr, c0);
 #pragma unroll
@@ -269,13 +321,19 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
       if (!inside(i)) continue;
       float v[8], u[8];
       x[e].get(v);
+      const auto magnitudes = [&](const float(&m)[8]) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(m[j]));
+        if constexpr (KEEP) {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) value[e][j] = m[j];
+        }
+      };
       if constexpr (OP == SILU_MUL) {
         y[e].get(u);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          value[e][j] = silu_mul(v[j], u[j]);
-          amax = max_nan(amax, fabsf(value[e][j]));
-        }
+        for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
+        magnitudes(v);
         continue;
       }
       if (OP == RESIDUAL) {
@@ -283,35 +341,32 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
         y[e].get(u);
         if (post) {
           factors(post, i, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) u[j] = u[j] * rd * f[j];
+          scale8<PAIRS>(u, rd);
+          mul8<PAIRS>(u, f);
         }
         if (gate) {
           factors(gate, i, f);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) u[j] *= f[j];
+          mul8<PAIRS>(u, f);
         }
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = fmaf(p.scale, u[j], v[j]);
+        add_scaled8<PAIRS>(v, p.scale, u);
         x[e].set(v);                                 // the value that is stored, which the norm reads
         x[e].template store<ALIGNED>(hidden, i, n);
         x[e].get(v);
       }
       if (NORMED) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(v[j], v[j], ss);
+        squares.template add<PAIRS>(v);
         if (QUANT) {
           factors(weight, i, u);
-#pragma unroll
-          for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j] * u[j]));
+          mul8<PAIRS>(v, u);
+          magnitudes(v);
         }
       } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) amax = max_nan(amax, fabsf(v[j]));
+        magnitudes(v);
       }
     }
   }
   if (!QUANT && !weight) return;                     // RESIDUAL without a norm after it
+  float ss = squares.template sum<PAIRS>();
   reduce_row<WARP_ROW>(ss, amax, red[1]);
   const float rr = NORMED ? rsqrtf(ss / static_cast<float>(n) + p.eps) : 1.0f;
   const bool finite = amax < __uint_as_float(0x7F800000u);       // (false for NaN)
@@ -327,19 +382,19 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
       const int i = i0 + c0 + e * per_octet;
       if (!inside(i)) continue;
       float v[8], u[8];
-      if constexpr (OP == SILU_MUL) {
-        if (!WHOLE) {
-          x[e].get(v);
-          y[e].get(u);
-        }
+      if constexpr (KEEP) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = WHOLE ? value[e][j] : silu_mul(v[j], u[j]);
+        for (int j = 0; j < 8; ++j) v[j] = value[e][j];
       } else {
         x[e].get(v);
-        if (NORMED) {
-          factors(weight, i, u);
+        if (OP == SILU_MUL) {
+          y[e].get(u);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = QUANT ? v[j] * u[j] : v[j] * rr * u[j];
+          for (int j = 0; j < 8; ++j) v[j] = silu_mul(v[j], u[j]);
+        } else if (NORMED) {
+          factors(weight, i, u);
+          if (!QUANT) scale8<PAIRS>(v, rr);
+          mul8<PAIRS>(v, u);
         }
       }
       if (QUANT) {
