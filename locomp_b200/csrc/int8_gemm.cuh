@@ -395,6 +395,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
   } else if (warp == WARP_MMA) {
     // ------------------------------------------------------------ MMA issuer: one warp for the team
+    griddep_wait();                            // (so that the limits of its waits count this kernel's time alone)
     if (crank == 0) {
       const uint32_t desc0 = gemm_tc::make_b_desc(smem_u32(smem));             // descriptors count 16-byte units
       Ring r = {0, 0}, rd = {0, 0};

@@ -93,8 +93,8 @@ def _empty_tokens(shape, device) -> QuantizedTokens:
     return QuantizedTokens(wide[..., :n], torch.empty(tuple(shape[:-1]), dtype=torch.float32, device=device))
 
 
-def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[QuantizedTokens, int]:
-    """The tokens a call writes, and how far apart their rows are."""
+def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[QuantizedTokens, int, int, int]:
+    """The tokens a call writes, the addresses of q and scales, and how far apart the rows of q are."""
     if out is None:
         out = _empty_tokens(shape, torch.device("cuda", dev))
     elif not isinstance(out, QuantizedTokens):
@@ -112,7 +112,7 @@ def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[Quanti
         raise TypeError("out must live on the device")
     if qo.device != dev or so.device != dev:
         raise ValueError("all operands must live on one device")
-    return out, ld
+    return out, qo.ptr, so.ptr, ld
 
 
 # ------------------------------------------------------------------------------------------ rows
@@ -120,7 +120,8 @@ def quantize_tokens(x, weight=None, eps: float = 1e-5, *, out: Optional[Quantize
                     bf16: bool = False) -> QuantizedTokens:
     """x ([n] or [rows, n]; rows may be further apart than n) as int8 tokens: scale = max|v| / 127 over a row, q = rint(v / scale),
     with v = x or, where `weight` is given, rms_norm(x, weight, eps).  A row of zeros has scale 1; a row that holds an infinity or a NaN
-    has scale NaN (and q 0), and so do all products with it.  Without `weight`: the values and scales of quantize(x, n, bits=8)."""
+    has scale NaN (and q 0), and so do all products with it.  Without `weight`: the values and scales of quantize(x, n, bits=8), but for
+    such rows and for scales that would be below 2**-126."""
     if stream is None and not bf16 and isinstance(x, torch.Tensor):
         res = _lib.calls.quantize_tokens(x, weight, eps, None if out is None else (out.q, out.scales))
         if res is not NotImplemented:
@@ -134,9 +135,9 @@ def quantize_tokens(x, weight=None, eps: float = 1e-5, *, out: Optional[Quantize
     code = _float_kind(xo, "x")
     _require_cuda()
     with _on(dev, stream):
-        t, ldq = _tokens_out(out, xo.shape, dev)
-        _lib.check(_lib.lib().lcq_quantize_tokens(xo.ptr, ldx, wo.ptr if wo else None, t.q.data_ptr(), ldq, t.scales.data_ptr(), rows, n,
-                                                  float(eps), code, current_stream_ptr()))
+        t, q_ptr, s_ptr, ldq = _tokens_out(out, xo.shape, dev)
+        _lib.check(_lib.lib().lcq_quantize_tokens(xo.ptr, ldx, wo.ptr if wo else None, q_ptr, ldq, s_ptr, rows, n, float(eps), code,
+                                                  current_stream_ptr()))
     return t
 
 
@@ -155,9 +156,8 @@ def silu_mul_tokens(gate, up, *, out: Optional[QuantizedTokens] = None, stream=N
     code = _float_kind(go, "gate")
     _require_cuda()
     with _on(dev, stream):
-        t, ldq = _tokens_out(out, go.shape, dev)
-        _lib.check(_lib.lib().lcq_silu_mul_tokens(go.ptr, ldg, uo.ptr, ldu, t.q.data_ptr(), ldq, t.scales.data_ptr(), rows, n, code,
-                                                  current_stream_ptr()))
+        t, q_ptr, s_ptr, ldq = _tokens_out(out, go.shape, dev)
+        _lib.check(_lib.lib().lcq_silu_mul_tokens(go.ptr, ldg, uo.ptr, ldu, q_ptr, ldq, s_ptr, rows, n, code, current_stream_ptr()))
     return t
 
 
@@ -212,8 +212,7 @@ def residual_norms(hidden, delta, weight=None, eps: float = 1e-5, *, post_weight
     with _on(dev, stream):
         oo, res, out_ptr, ldo, scales = None, new_hidden, None, n, None
         if quantized:
-            res, ldo = _tokens_out(out, ho.shape, dev)
-            out_ptr, scales = res.q.data_ptr(), res.scales.data_ptr()
+            res, out_ptr, scales, ldo = _tokens_out(out, ho.shape, dev)
         elif weight is not None:
             res = torch.empty(ho.shape, dtype=KIND_TO_TORCH[kind], device=torch.device("cuda", dev)) if out is None else out
             oo = resolve(res, "out", bf16)

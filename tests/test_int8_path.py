@@ -544,6 +544,60 @@ def test_row_refusals():
     status_ok()
 
 
+@pytest.mark.gpu
+def test_tokens_into_other_objects():
+    """Outputs given as this package's tensors; the general path writes where the native one does."""
+    x = torch.randn(6, 100, device="cuda", generator=gen(9)).half()
+    q, s = L.empty((6, 112), dtype="int8"), L.empty(6)
+    want = L.quantize_tokens(x)
+    with pytest.raises(ValueError, match="out.q"):
+        L.quantize_tokens(x, out=L.QuantizedTokens(q, s))                 # rows of 112
+    t = L.QuantizedTokens(L.DeviceTensor(torch.empty(6, 100, dtype=torch.int8, device="cuda")), s)
+    assert L.quantize_tokens(x, out=t) is t and torch.equal(t.q.torch(), want.q) and torch.equal(s.torch(), want.scales)
+    assert L.silu_mul_tokens(x, x, out=t) is t and torch.equal(t.q.torch(), L.silu_mul_tokens(x, x).q)
+    w = torch.ones(100, device="cuda").half()
+    assert L.residual_norms(x.clone(), x, w, quantized=True, out=t) is t
+    with pytest.raises(TypeError, match="device"):
+        L.quantize_tokens(x, out=L.QuantizedTokens(want.q.cpu().numpy().copy(), s))
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """Rows, weights and outputs of more than 2^31 values: the last ones are where they belong."""
+    n, rows = 32768, 66000                                                # 2.16e9 values
+    x = torch.empty(rows, n, dtype=torch.bfloat16, device="cuda")
+    x[:] = torch.randn(1, n, device="cuda", generator=gen(10))
+    x[-3:] *= torch.tensor([[2.0], [0.0], [3.0]], device="cuda", dtype=torch.bfloat16)
+    t = L.quantize_tokens(x)
+    small = L.quantize_tokens(x[-4:].contiguous())
+    assert torch.equal(t.q[-4:], small.q) and torch.equal(t.scales[-4:], small.scales) and torch.equal(t.q[0], t.q[rows // 2])
+    w = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    out = torch.empty_like(x)
+    L.residual_norms(x, x, w, hidden_out=out, out=out)                    # (out twice: the norm is what stays)
+    h = x[-4:].float() + x[-4:].float()
+    ref = L.rms_norm(h.to(torch.bfloat16), w)
+    assert bool(((out[-4:].double() - ref.double()).abs() <= 2.0 ** -7 * ref.double().abs()).all())
+    del out, x
+    k = 64
+    a, xs, b, ws, _ = product_case(rows, n, k)
+    y = L.int8_matmul(a, xs, b, ws)                                       # 2.16e9 outputs
+    check_product(y[-5:], a[-5:].double() @ b.double().t() * xs[-5:].double()[:, None] * ws.double(), torch.float16)
+    check_product(y[:5], a[:5].double() @ b.double().t() * xs[:5].double()[:, None] * ws.double(), torch.float16)
+    del y
+    wide = torch.randint(-128, 128, (300000, 8192), dtype=torch.int8, device="cuda", generator=gen(11))          # 2.46e9 weights
+    scales = torch.rand(300000, device="cuda", generator=gen(12)) * 0.01
+    for m in (1, 5, 16, 70):
+        x8, xs, _, _, _ = product_case(m, 8, 8192)
+        y = L.int8_matmul(x8, xs, wide, scales, out_dtype="f32")
+        check_product(y[:, -300:], x8.double() @ wide[-300:].double().t() * xs.double()[:, None] * scales[-300:].double(), torch.float32)
+    odd = wide.view(-1)[:300000 * 8191].view(300000, 8191)                # rows off 16 bytes, 51 pieces
+    y = L.int8_matmul(x8[:, :8191], xs, odd, scales, out_dtype="f32")
+    check_product(y[:, -300:], x8[:, :8191].double() @ odd[-300:].double().t() * xs.double()[:, None] * scales[-300:].double(), torch.float32)
+    y = L.int8_matmul(x8[:3, :8191], xs[:3], odd, scales, out_dtype="f32")
+    check_product(y[:, -300:], x8[:3, :8191].double() @ odd[-300:].double().t() * xs[:3].double()[:, None] * scales[-300:].double(), torch.float32)
+    status_ok()
+
+
 # ------------------------------------------------------------------------------------------ together
 @pytest.mark.gpu
 @pytest.mark.parametrize("m,hidden,inter", [(1, 576, 1536), (5, 200, 333), (16, 512, 1024), (130, 264, 700)])
