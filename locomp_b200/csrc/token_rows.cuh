@@ -97,17 +97,19 @@ template <typename T> struct Raw<T, false> {
     uint32_t w[4 * W + 4];
 #pragma unroll
     for (int j = 0; j <= W; ++j) { w[4 * j] = r[j].x; w[4 * j + 1] = r[j].y; w[4 * j + 2] = r[j].z; w[4 * j + 3] = r[j].w; }
-    if (off & 8) {
+    if (S == 4 || off) {                             // (the same for a whole row; in float32 the branch costs registers that are short)
+      if (off & 8) {
 #pragma unroll
-      for (int j = 0; j < 4 * W + 2; ++j) w[j] = w[j + 2];
-    }
-    if (off & 4) {
+        for (int j = 0; j < 4 * W + 2; ++j) w[j] = w[j + 2];
+      }
+      if (off & 4) {
 #pragma unroll
-      for (int j = 0; j < 4 * W + 1; ++j) w[j] = w[j + 1];
-    }
-    if (S == 2) {
+        for (int j = 0; j < 4 * W + 1; ++j) w[j] = w[j + 1];
+      }
+      if (S == 2) {
 #pragma unroll
-      for (int j = 0; j < 4 * W; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 2) * 8);
+        for (int j = 0; j < 4 * W; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], (off & 2) * 8);
+      }
     }
     if (i < 0 || i + 8 > n) {
 #pragma unroll
@@ -424,7 +426,8 @@ int launch_form(const Args& p, int threads, cudaStream_t st) {
 //   E = 1, most threads a row         few rows, where latency counts (1 x 4096: 2.6; E = 2 3.2, E = 4 4.4), and RESIDUAL up to 2048 values or 8 Mi in all
 //   E = 4, most bytes on their way    all other 16-bit rows up to 16,384 (8192 x 8192 RESIDUAL: 87; E = 1 122, E = 2 98, E = 8 101)
 //   E = 2                             float32, and rows off 16 bytes, which hold more registers for each octet (4000 x 5003: 48; E = 1 59, E = 4 56)
-//   E = 8                             16-bit rows up to 32,768 (1000 x 28,672 SILU_MUL: 45; in chunks 58)
+//   E = 8                             16-bit rows up to 32,768 of one operand (4000 x 28,672 quantised: 69; E = 4 93); of two, E = 4 in twice the threads
+//                                     (1000 x 28,672 SILU_MUL: 39; E = 8 44, in chunks 58)
 template <typename T, int OP, bool QUANT, bool ALIGNED>
 int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
   constexpr bool HALF = sizeof(T) == 2, ONE = OP == ROWS || OP == NORM_ROWS;
@@ -444,7 +447,11 @@ int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
     if (span <= 16384) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 512, ONE ? 3 : 2>(p, threads(4), st);
   }
   if constexpr (HALF) {
-    if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 8, false, true, 512, ONE ? 2 : 1>(p, threads(8), st);
+    if constexpr (ONE) {
+      if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 8, false, true, 512, 2>(p, threads(8), st);
+    } else {
+      if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 1024, 1>(p, threads(4), st);
+    }
   }
   return launch_form<T, OP, QUANT, ALIGNED, 2, false, false, 512, 2>(p, 512, st);
 }
