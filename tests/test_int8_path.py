@@ -194,6 +194,20 @@ def test_product_writes_its_rows_and_nothing_else():
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("m,n,k", [(300, 257, 64), (77, 258, 640), (130, 131, 33), (64, 516, 32), (257, 391, 144), (1000, 255, 272), (33, 1029, 16), (150, 384, 96), (600, 3001, 128)])
+def test_product_at_every_place_in_16_bytes(m, n, k, kind):
+    x, xs, w, ws, ref = product_case(m, n, k)
+    for place in range(16 // kind.itemsize):
+        buf = torch.full((m * n + 64,), -7.0, dtype=kind, device="cuda")
+        out = buf[16 + place:16 + place + m * n].view(m, n)
+        assert L.int8_matmul(x, xs, w, ws, out=out) is out
+        check_product(out, ref, kind)
+        assert bool((buf[:16 + place] == -7).all()) and bool((buf[16 + place + m * n:] == -7).all())
+    status_ok()
+
+
+@pytest.mark.gpu
 def test_product_of_weights_that_the_kernel_ahead_writes():
     """No synchronisation between what writes the operands and the product: 64 rounds with other weights each time."""
     m, n, k = 4, 8192, 2048
