@@ -312,23 +312,36 @@ PyObject* add_inplace(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return finish(unlocked([&] { return api.add_inplace(a->data_ptr(), b->data_ptr(), a->numel(), code, stream); }), args[0]);
 }
 
-// A CUDA tensor whose rows (its last dimension) are contiguous and equally far apart, `ld` elements; or nullptr.
+// Elements between the rows (last dimension) of a tensor whose rows are contiguous, equally far apart and apart from each other; or -1.
+int64_t row_stride_of(const at::Tensor& t) {
+  const int64_t n = t.size(-1);
+  if (t.is_contiguous()) return n;
+  if (n != 1 && t.stride(-1) != 1) return -1;
+  int64_t ld = n, span = -1;             // what the dimensions seen so far span; -1: none yet (a broadcast one spans 0)
+  for (int64_t d = t.dim() - 2; d >= 0; --d) {
+    if (t.size(d) == 1) continue;
+    if (span < 0) ld = t.stride(d);
+    else if (t.stride(d) != span) return -1;
+    if (ld < n) return -1;
+    span = t.stride(d) * t.size(d);
+  }
+  return ld;
+}
+// A CUDA tensor of such rows, `ld` elements apart; or nullptr.
 const at::Tensor* row_tensor(PyObject* o, int64_t& ld) {
   if (!THPVariable_CheckExact(o)) return nullptr;
   const at::Tensor& t = THPVariable_Unpack(o);
   if (!t.is_cuda() || t.layout() != at::kStrided || t.dim() < 1 || t.numel() == 0) return nullptr;
-  const int64_t n = t.size(-1);
-  ld = n;
-  if (t.is_contiguous()) return &t;
-  if (n != 1 && t.stride(-1) != 1) return nullptr;
-  int64_t span = 0;                      // of the dimensions seen so far
-  for (int64_t d = t.dim() - 2; d >= 0; --d) {
-    if (t.size(d) == 1) continue;
-    if (span == 0) ld = t.stride(d);
-    else if (t.stride(d) != span) return nullptr;
-    span = t.stride(d) * t.size(d);
-  }
-  return ld >= n ? &t : nullptr;
+  ld = row_stride_of(t);
+  return ld < 0 ? nullptr : &t;
+}
+// row_stride(tensor) -> elements between its rows, or None
+PyObject* row_stride(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  if (n_args != 1 || !THPVariable_Check(args[0])) return not_implemented();
+  const at::Tensor& t = THPVariable_Unpack(args[0]);
+  const int64_t ld = t.layout() == at::kStrided && t.dim() > 0 ? row_stride_of(t) : -1;
+  if (ld < 0) Py_RETURN_NONE;
+  return PyLong_FromLongLong(ld);
 }
 // The int8 rows and scales that a call writes: new ones, or the tensors of the pair `given`.
 struct Tokens {
@@ -692,6 +705,7 @@ PyMethodDef methods[] = {
     LCQ_METHOD(matmul), LCQ_METHOD(dequantize), LCQ_METHOD(quantize), LCQ_METHOD(rms_norm), LCQ_METHOD(residual_rms_norm),
     LCQ_METHOD(silu_mul), LCQ_METHOD(add_inplace), LCQ_METHOD(embed_lookup), LCQ_METHOD(argmax), LCQ_METHOD(set_workspace),
     LCQ_METHOD(quantize_tokens), LCQ_METHOD(silu_mul_tokens), LCQ_METHOD(residual_norms), LCQ_METHOD(int8_matmul),
+    LCQ_METHOD(row_stride),
     LCQ_METHOD(lock_workspace), LCQ_METHOD(unlock_workspace),
     {"bind", bind, METH_VARARGS, nullptr},
     {nullptr, nullptr, 0, nullptr}};

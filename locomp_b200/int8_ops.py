@@ -51,28 +51,10 @@ def _on(device: int, stream):
             yield
 
 
-def _row_stride(t: torch.Tensor) -> Optional[int]:
-    """Elements between the rows (last dimension) of a tensor whose rows are contiguous and equally far apart, else None."""
-    n = t.shape[-1]
-    if n != 1 and t.stride(-1) != 1:
-        return None
-    ld = span = None
-    for size, stride in reversed(list(zip(t.shape[:-1], t.stride()[:-1]))):
-        if size == 1:
-            continue
-        if ld is None:
-            ld, span = stride, stride * size
-        elif stride != span:
-            return None
-        else:
-            span = stride * size
-    return n if ld is None else ld if ld >= n else None
-
-
 def _resolve_rows(arg, name: str, bf16: bool = False) -> Tuple[Operand, int]:
     """An operand whose rows may be further apart than they are long (torch tensors only), and how far."""
     if isinstance(arg, torch.Tensor) and arg.is_cuda and arg.dim() > 0 and arg.numel() and not arg.is_contiguous():
-        ld = _row_stride(arg)
+        ld = _lib.calls.row_stride(arg)
         if ld is not None:
             one_row = resolve(arg[(0,) * (arg.dim() - 1)].reshape(-1), name, bf16)      # (checks the type)
             return Operand(arg.data_ptr(), one_row.kind, tuple(arg.shape), arg.numel(), arg.device.index, arg), ld

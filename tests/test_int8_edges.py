@@ -1,0 +1,90 @@
+"""The int8 path where its calls go wrong most easily: views, broadcast dimensions, sizes at the ends of the range.
+
+Bounds are those of test_int8_path.py: a product is an exact integer, three float32 roundings and the output's own; a normalised value
+is good to REL = 2^-18."""
+import itertools
+
+import pytest
+import torch
+
+import locomp_b200 as L
+from locomp_b200 import _lib
+from test_int8_path import HALF_STEP, KINDS, NAMES, REL, check_product, check_tokens, gen, product_case, rms, status_ok
+
+
+# ------------------------------------------------------------------------------------------ views
+def rows_apart(t):
+    """By listing where every row starts: the distance between rows, where there is one that keeps them apart."""
+    n = t.shape[-1]
+    if n != 1 and t.stride(-1) != 1:
+        return None
+    starts = [sum(i * s for i, s in zip(at, t.stride())) for at in itertools.product(*map(range, t.shape[:-1]))]
+    if len(starts) == 1:
+        return n
+    ld = starts[1] - starts[0]
+    return ld if ld >= n and starts == [i * ld for i in range(len(starts))] else None
+
+
+def test_row_stride_is_that_of_every_row():
+    views = 0
+    for shape in ((8,), (3, 8), (3, 4, 8), (2, 3, 2, 4), (3, 1, 8), (1, 3, 8), (3, 4, 1), (1, 1, 8)):
+        steps = [(0, 1, 4, 8, 12, 16, 24, 32, 48, 96)] * (len(shape) - 1) + [(1, 2)]
+        for strides in itertools.product(*steps):
+            t = torch.empty(4096, dtype=torch.int8).as_strided(shape, strides)
+            got, want = _lib.calls.row_stride(t), rows_apart(t)
+            if all(s == 1 for s in shape[:-1]):           # a single row: any distance serves
+                want = None if want is None else got
+            assert got == want, (shape, strides, got, want)
+            views += got is not None
+    assert views > 50
+    base = torch.zeros(3, 8)
+    assert _lib.calls.row_stride(base[:, None].expand(3, 4, 8)) is None
+    assert _lib.calls.row_stride(base[None].expand(4, 3, 8)) is None
+    assert _lib.calls.row_stride(base[:, None, None].expand(3, 2, 2, 8)) is None
+    assert _lib.calls.row_stride(base[:, :5]) == 8 and _lib.calls.row_stride(base[:, None]) == 8
+    assert _lib.calls.row_stride(base.t()) is None and _lib.calls.row_stride(torch.zeros(())) is None
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_broadcast_rows_are_refused(kind):
+    """Twelve rows of a storage that is cut out of a larger one, so that no stride leads out of it."""
+    whole = torch.randn(64, 64, device="cuda", generator=gen(1)).to(kind)
+    base = whole[:3, :]
+    good = whole[:12].view(3, 4, 64)
+    for x in (base[:, None].expand(3, 4, 64), base[None].expand(4, 3, 64), base[:1, None].expand(1, 4, 64)):
+        with pytest.raises(ValueError, match="contiguous"):
+            L.quantize_tokens(x)
+        for gate, up in ((x, x), (good.reshape(x.shape) if x.numel() == good.numel() else x, x)):
+            with pytest.raises(ValueError, match="contiguous"):
+                L.silu_mul_tokens(gate, up)
+    q = torch.full((64, 64), 5, dtype=torch.int8, device="cuda")
+    s = torch.zeros(3, 4, device="cuda")
+    w = torch.ones(64, device="cuda", dtype=kind)
+    for out_q in (q[:3, None].expand(3, 4, 64), q[None, :4].expand(3, 4, 64)):
+        t = L.QuantizedTokens(out_q, s)
+        with pytest.raises(ValueError, match="contiguous"):
+            L.quantize_tokens(good, out=t)
+        with pytest.raises(ValueError, match="contiguous"):
+            L.silu_mul_tokens(good, good, out=t)
+        with pytest.raises(ValueError, match="contiguous"):
+            L.residual_norms(good.clone(), good, w, quantized=True, out=t)
+    assert bool((q == 5).all()) and bool((s == 0).all())
+    status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_views_of_three_dimensions(kind):
+    """Rows equally far apart over two dimensions are read and written where they are."""
+    whole = torch.randn(3, 4, 80, device="cuda", generator=gen(2)).to(kind)
+    x = whole[..., 8:72]
+    t, want = L.quantize_tokens(x), L.quantize_tokens(x.contiguous())
+    assert t.q.shape == (3, 4, 64) and torch.equal(t.q, want.q) and torch.equal(t.scales, want.scales)
+    q = torch.full((3, 4, 96), 7, dtype=torch.int8, device="cuda")
+    out = L.QuantizedTokens(q[..., :64], torch.empty(3, 4, device="cuda"))
+    assert L.quantize_tokens(x, out=out) is out and torch.equal(out.q, want.q) and bool((q[..., 64:] == 7).all())
+    s = L.silu_mul_tokens(x, x)
+    assert torch.equal(s.q, L.silu_mul_tokens(x.contiguous(), x.contiguous()).q)
+    with pytest.raises(ValueError, match="contiguous"):
+        L.quantize_tokens(whole[:, :3, :64])          # four rows a block in storage, three of them taken: not equally far apart
