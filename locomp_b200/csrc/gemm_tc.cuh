@@ -530,13 +530,15 @@ w4a16_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_const
     mbar_init(drained, 1);
     *flag_abort = 0;
     fence_barrier_init();
-    griddep_launch_dependents();
   }
   if (warp == WARP_MMA) tmem_alloc<CG>(tmem_slot, TMEM_COLS);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   if (CG == 2) cluster_barrier();             // the other CTA's barriers exist
+  // The next kernel starts once all CTAs have come here, with their columns of tensor memory.  A CTA waits for its columns without a limit: were a successor
+  // let onto the SM before, it could take them and then wait for this kernel to end, which waits for them.
+  if (threadIdx.x == 0) griddep_launch_dependents();
   const uint32_t tmem_base = *tmem_slot;
   const uint32_t a_base = tmem_base + TMEM_COLS - p.nas * A_SLOT_COLS;
 

@@ -349,7 +349,6 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     mbar_init(drained, 1);
     *flag_abort = 0;
     fence_barrier_init();
-    griddep_launch_dependents();
   }
   if (warp == WARP_TMA && lane == 0) {
     tma_prefetch_desc(&tmap_w);
@@ -365,6 +364,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
   __syncthreads();
   tc_fence_after();
   if (CG == 2) cluster_barrier();             // the other CTA's barriers exist
+  if (threadIdx.x == 0) griddep_launch_dependents();       // after tmem_alloc: see gemm_tc.cuh
   const uint32_t tmem_base = *tmem_slot;
 
 #define LCQ_GIVE_UP(code)                                                                              \
@@ -750,6 +750,16 @@ inline Params make_params(const Tiling& t, int M, int N, int K) {
   return p;
 }
 
+// The shared memory of a launch.  A CTA waits without a limit for its columns of tensor memory, and the other CTAs of its cluster wait for it: two clusters
+// of two streams that meet on two SMs in opposite order, each with columns that the other one wants, would wait for good.  So a cluster's CTAs take as much of an
+// SM's 228 KB as of its 512 columns, and a little more: where the columns of several are too many, they do not fit on an SM together.
+// (Asked for beyond the ring by pairs with K of 384 and less.)
+constexpr int SMEM_PER_COLUMN = 440;           // 544 columns (the least that is too many): 233.75 KB
+inline int launch_smem(const Params& p, int cg) {
+  const int ring = smem_map(p.bm, cg, p.depth).total, columns = cg * p.split > 1 ? p.tmem_cols * SMEM_PER_COLUMN : 0;
+  return ring > columns ? ring : columns;
+}
+
 template <int CG, typename OT>
 int launch_t(const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
   auto kern = int8_gemm_kernel<CG, OT>;
@@ -762,7 +772,7 @@ int launch_t(const CUtensorMap* tm, const Params& p, cudaStream_t stream) {
   }
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[2];
-  gemm_tc::pdl_launch_config(cfg, attr, CG * p.teams, NTHREADS, smem_map(p.bm, CG, p.depth).total, stream);
+  gemm_tc::pdl_launch_config(cfg, attr, CG * p.teams, NTHREADS, launch_smem(p, CG), stream);
   const int cluster = CG == 2 ? 2 : p.split;
   if (cluster > 1) {
     cudaLaunchAttribute& a = attr[cfg.numAttrs++];

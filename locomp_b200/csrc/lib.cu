@@ -777,7 +777,7 @@ size_t lcq_int8_matmul_workspace_bytes(int M, int N, int K, int x_on_16, int w_o
 static int check_int8_tiling(const int8_gemm::Tiling& t, int M, int N, int K, int sm_count) {
   using namespace int8_gemm;
   const Params p = make_params(t, M, N, K);
-  const int smem = smem_map(p.bm, t.cg, p.depth).total;
+  const int smem = launch_smem(p, t.cg);
   const auto wrong = [](const char* what) { set_error("int8 plan: %s", what); return LCQ_ERR_BAD_ARG; };
   if (smem > 227 * 1024 || t.depth < 2 || t.depth > MAX_STAGES) return wrong("shared memory");
   if (t.bm % (16 * t.cg) != 0 || t.bm > 256 || p.tmem_cols > 512 || t.bm + (t.bm + 31) / 32 * 32 > p.tmem_cols) return wrong("tensor memory");
@@ -817,7 +817,7 @@ int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int w_on_16, i
   }
   if (fields) {
     const Tiling& t = q.main;
-    const int f[9] = {t.cg * t.teams, t.bm, t.n_tiles, t.tail > 1 ? t.n_tiles - t.full : 0, smem_map(t.bm, t.cg, t.depth).total, t.cg, t.split, t.depth, q.piece};
+    const int f[9] = {t.cg * t.teams, t.bm, t.n_tiles, t.tail > 1 ? t.n_tiles - t.full : 0, launch_smem(make_params(t, M, q.piece, K), t.cg), t.cg, t.split, t.depth, q.piece};
     memcpy(fields, f, sizeof(f));
   }
   return check_int8_tiling(q.main, M, q.piece, K, sm_count);

@@ -3,13 +3,15 @@
 Bounds are those of test_int8_path.py: a product is an exact integer, three float32 roundings and the output's own; a normalised value
 is good to REL = 2^-18."""
 import itertools
+import os
+import random
 
 import pytest
 import torch
 
 import locomp_b200 as L
 from locomp_b200 import _lib
-from test_int8_path import HALF_STEP, KINDS, NAMES, REL, check_product, check_tokens, gen, product_case, rms, status_ok
+from test_int8_path import HALF_STEP, KINDS, NAMES, REL, check_product, check_tokens, gen, plan, product_case, rms, status_ok
 
 
 # ------------------------------------------------------------------------------------------ views
@@ -88,3 +90,58 @@ def test_views_of_three_dimensions(kind):
     assert torch.equal(s.q, L.silu_mul_tokens(x.contiguous(), x.contiguous()).q)
     with pytest.raises(ValueError, match="contiguous"):
         L.quantize_tokens(whole[:, :3, :64])          # four rows a block in storage, three of them taken: not equally far apart
+
+
+# ------------------------------------------------------------------------------------------ kernels that share an SM
+def test_no_successor_before_the_tensor_memory_is_taken():
+    """A CTA that waits for columns of tensor memory must not have let the next kernel onto its SM: order of the source, since running
+    it the other way round may hang a GPU."""
+    for name in ("gemm_tc.cuh", "int8_gemm.cuh"):
+        text = open(os.path.join(os.path.dirname(_lib.__file__), "csrc", name)).read()
+        kernel = text[text.index("extern __shared__"):]
+        kernel = kernel[:kernel.index("\n}\n")]
+        places = [kernel.index(s) for s in ("tmem_alloc<CG>(tmem_slot", "__syncthreads();", "cluster_barrier();", "griddep_launch_dependents();")]
+        assert places == sorted(places), name
+        assert kernel.count("griddep_launch_dependents") == 1 and kernel.count("tmem_alloc<") == 1
+
+
+def test_clusters_that_fit_on_an_sm_fit_into_its_tensor_memory():
+    """Two clusters that meet on two SMs in opposite order, and do not fit there together, would wait for each other."""
+    seen = {}
+    r = random.Random(5)
+    problems = [(692, 7513, 114), (412, 6844, 53), (38, 2663, 2811), (2049, 3000, 256), (512, 14336, 128)]
+    problems += [(int(2 ** r.uniform(3, 11)), int(2 ** r.uniform(5, 13)), int(2 ** r.uniform(5, 12))) for _ in range(3000)]
+    for m, n, k in problems:
+        p = plan(m, n, k)
+        if p["cg"] * p["split"] == 1:
+            continue
+        columns = 32
+        while columns < p["bm"] + (p["bm"] + 31) // 32 * 32:          # two accumulators, the second read 32 columns at a time
+            columns *= 2
+        seen[columns] = min(seen.get(columns, 1 << 30), p["smem"] + 1024)      # 1 KB of a CTA is the system's
+    assert 512 in seen and len(seen) > 2
+    most = 228 * 1024
+    for counts in itertools.product(*(range(most // s + 1) for s in seen.values())):
+        if sum(c * s for c, s in zip(counts, seen.values())) <= most:
+            assert sum(c * k for c, k in zip(counts, seen)) <= 512, (seen, counts)
+
+
+@pytest.mark.gpu
+def test_small_and_large_products_in_a_chain_and_on_two_streams():
+    """Short rings, which leave room on an SM, one after the other and side by side."""
+    sizes = [(16, 16384, 128), (1000, 3000, 128), (692, 7513, 114), (16, 16384, 128), (2048, 512, 144), (40, 2663, 2816)]
+    cases = [product_case(*s) for s in sizes]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(60):
+        outs.append((i % 6, L.int8_matmul(*cases[i % 6][:4], out_dtype="f32")))
+    for i in range(60):
+        outs.append((i // 2 % 6, L.int8_matmul(*cases[i // 2 % 6][:4], out_dtype="f32", stream=streams[i % 2])))
+    torch.cuda.synchronize()
+    first = {}
+    for i, y in outs:
+        if i not in first:
+            check_product(y, cases[i][4], torch.float32)
+        assert torch.equal(first.setdefault(i, y), y)
+    status_ok()
