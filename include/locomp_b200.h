@@ -178,7 +178,7 @@ int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
  * lcq_int8_matmul: out[m, n] = (sum_k x[m, k] * w[n, k]) * x_scales[m] * w_scales[n].
  *   x int8 [M, K] with rows ldx bytes apart, x_scales float32 [M]; w int8 [N, K] with rows ldw bytes apart, w_scales [N] of
  *   w_scale_dtype (lcq_quantize_int8 with group_size = K makes both); out [M, N] of out_dtype, contiguous.  The sum is an exact
- *   int32 (K <= 131071, else LCQ_ERR_UNSUPPORTED), the scales are applied in float32, the result is rounded once.  Rows on 16 bytes
+ *   int32 (K <= 131071, M and N <= 2000000000, else LCQ_ERR_UNSUPPORTED), the scales are applied in float32, the result is rounded once.  Rows on 16 bytes
  *   (x, w, ldx, ldw multiples of 16; ld does not matter to a single row) are read where they are, any other are first copied into the
  *   workspace: x whole, w at most 48 MiB at a time.
  *   workspace: of lcq_int8_matmul_workspace_bytes() bytes, 256-byte aligned, for those copies (none: NULL); it need not be cleared, and a buffer of

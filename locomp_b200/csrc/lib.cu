@@ -704,6 +704,10 @@ static int64_t stride_of(int64_t rows, int64_t ld, int64_t n) { return rows > 1 
 static int check_int8_problem(int M, int N, int K) {
   if (M < 0 || N < 0 || K <= 0) { set_error("int8 matmul: bad sizes M=%d N=%d K=%d", M, N, K); return LCQ_ERR_BAD_ARG; }
   if (K > int8_gemm::MAX_K) { set_error("int8 matmul: K=%d is more than int32 sums hold (%d)", K, int8_gemm::MAX_K); return LCQ_ERR_UNSUPPORTED; }
+  if (M > 2000000000 || N > 2000000000) {      // (a tile's rows and channels are counted in int, up to 256 past the last one)
+    set_error("int8 matmul: M=%d by N=%d: at most 2000000000 of either are supported", M, N);
+    return LCQ_ERR_UNSUPPORTED;
+  }
   if ((static_cast<int64_t>(M) + 15) / 16 * ((static_cast<int64_t>(N) + 127) / 128) > (1 << 30)) {
     set_error("int8 matmul: M=%d by N=%d is more than 2^30 tiles", M, N);
     return LCQ_ERR_UNSUPPORTED;

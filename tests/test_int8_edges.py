@@ -2,6 +2,7 @@
 
 Bounds are those of test_int8_path.py: a product is an exact integer, three float32 roundings and the output's own; a normalised value
 is good to REL = 2^-18."""
+import ctypes
 import itertools
 import os
 import random
@@ -145,3 +146,15 @@ def test_small_and_large_products_in_a_chain_and_on_two_streams():
             check_product(y, cases[i][4], torch.float32)
         assert torch.equal(first.setdefault(i, y), y)
     status_ok()
+
+
+# ------------------------------------------------------------------------------------------ sizes
+def test_sizes_near_the_end_of_int_are_refused():
+    """Within a tile of 2^31 the kernels' channel and token numbers would pass the end of int."""
+    lib, f, p = _lib.lib(), (ctypes.c_int * 9)(), ctypes.c_void_p(4096)
+    for m, n in ((1, 2000000000), (2000000000, 1)):
+        assert lib.lcq_int8_matmul_workspace_bytes(m, n, 16, 1, 1) != (1 << 64) - 1
+    for m, n in ((1, 2000000001), (1, 2 ** 31 - 1), (2 ** 31 - 1, 1), (2 ** 31 - 1, 2 ** 31 - 1)):
+        assert lib.lcq_int8_matmul_workspace_bytes(m, n, 16, 1, 1) == (1 << 64) - 1
+        assert lib.lcq_int8_matmul_plan_check(m, n, 16, 148, 1, f) == _lib.ERR_UNSUPPORTED
+        assert lib.lcq_int8_matmul(p, 16, p, p, 16, p, p, m, n, 16, 0, 0, None, 0, None) == _lib.ERR_UNSUPPORTED
