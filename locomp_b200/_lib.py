@@ -14,8 +14,20 @@ ERR_BAD_ARG, ERR_UNSUPPORTED, ERR_CUDA, ERR_WORKSPACE, ERR_TIMEOUT = -1, -2, -3,
 F32, F16, BF16 = 0, 1, 2
 ALGO_AUTO, ALGO_SIMT, ALGO_GEMV_TC, ALGO_GEMM_TC, ALGO_GEMV_W8 = 0, 1, 2, 3, 4
 
-# name -> (restype, argtypes); mirrors include/locomp_b200.h one to one
 _c = ctypes
+
+
+class _Int:
+    """A C int as an argument type: ctypes.c_int would cut a larger number to 32 bits without a word."""
+
+    @staticmethod
+    def from_param(v):
+        if isinstance(v, int) and not -(1 << 31) <= v < 1 << 31:
+            raise ValueError(f"{v} does not fit a C int")
+        return _c.c_int.from_param(v)
+
+
+# name -> (restype, argtypes); mirrors include/locomp_b200.h one to one
 
 
 class DecodeStackDesc(_c.Structure):
@@ -104,7 +116,7 @@ def lib() -> ctypes.CDLL:
         for name, (res, args) in SIGNATURES.items():
             fn = getattr(handle, name)   # AttributeError if the symbol is not exported
             fn.restype = res
-            fn.argtypes = args
+            fn.argtypes = [_Int if a is _c.c_int else a for a in args]
         _lib = handle
     return _lib
 

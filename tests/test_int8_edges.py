@@ -158,3 +158,31 @@ def test_sizes_near_the_end_of_int_are_refused():
         assert lib.lcq_int8_matmul_workspace_bytes(m, n, 16, 1, 1) == (1 << 64) - 1
         assert lib.lcq_int8_matmul_plan_check(m, n, 16, 148, 1, f) == _lib.ERR_UNSUPPORTED
         assert lib.lcq_int8_matmul(p, 16, p, p, 16, p, p, m, n, 16, 0, 0, None, 0, None) == _lib.ERR_UNSUPPORTED
+
+
+def test_sizes_that_an_int_does_not_hold_are_refused():
+    """ctypes cuts an int to 32 bits: 2^32 + 8 values a row would run as 8, the others left as they were."""
+    lib, p, big = _lib.lib(), ctypes.c_void_p(4096), 2 ** 32
+    calls = [lambda: lib.lcq_int8_matmul(p, 16, p, p, 16, p, p, big, 0, 16, 0, 0, None, 0, None),
+             lambda: lib.lcq_int8_matmul_workspace_bytes(0, big + 8, 16, 1, 1),
+             lambda: lib.lcq_quantize_tokens(p, 8, None, p, 8, p, 0, big + 8, 1e-5, 0, None),
+             lambda: lib.lcq_silu_mul_tokens(p, 8, p, 8, p, 8, p, 0, -big, 0, None),
+             lambda: lib.lcq_residual_norms(p, p, None, None, 0, 1.0, None, p, None, 8, None, 0, big + 8, 1e-5, 0, None),
+             lambda: lib.lcq_rms_norm(p, p, p, 0, 2 ** 31, 1e-5, 0, None)]
+    for call in calls:
+        with pytest.raises(ctypes.ArgumentError, match="does not fit"):
+            call()
+    assert lib.lcq_quantize_tokens(None, 0, None, None, 0, None, big, 0, 1e-5, 0, None) == 0          # rows are 64 bits
+
+
+@pytest.mark.gpu
+def test_rows_that_an_int_does_not_hold_are_refused():
+    n = 2 ** 32 + 8
+    x = torch.zeros(1, n, dtype=torch.float16, device="cuda")
+    for call in (lambda: L.quantize_tokens(x), lambda: L.silu_mul_tokens(x, x), lambda: L.residual_norms(x, x)):
+        with pytest.raises(ctypes.ArgumentError, match="does not fit"):
+            call()
+    q = x.view(torch.int8)[:, :n]
+    one = torch.ones(1, device="cuda")
+    with pytest.raises(ctypes.ArgumentError, match="does not fit"):
+        L.int8_matmul(q, one, q, one)
