@@ -27,9 +27,6 @@ class _Int:
         return _c.c_int.from_param(v)
 
 
-# name -> (restype, argtypes); mirrors include/locomp_b200.h one to one
-
-
 class DecodeStackDesc(_c.Structure):
     """lcq_decode_stack."""
     _fields_ = ([(n, _c.c_void_p) for n in ("layers", "head_w", "head_s", "logits", "norms", "outputs", "token", "table", "x_q",
@@ -38,6 +35,7 @@ class DecodeStackDesc(_c.Structure):
                 [("eps", _c.c_float)])
 
 
+# name -> (restype, argtypes); mirrors include/locomp_b200.h one to one
 SIGNATURES = {
     "lcq_version": (_c.c_int, []),
     "lcq_status_string": (_c.c_char_p, [_c.c_int]),

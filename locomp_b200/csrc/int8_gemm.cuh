@@ -721,7 +721,9 @@ inline Plan make_plan(int M, int N, int K, int sm_count, const ClusterFit& fit, 
   memset(&q, 0, sizeof(q));
   q.piece = N;
   if (!w_mappable && N * row > W_COPY) {
-    const long long pieces = (N * row + W_COPY - 1) / W_COPY, rows = ((N + pieces - 1) / pieces + 255) / 256 * 256;
+    const long long pieces = (N * row + W_COPY - 1) / W_COPY;
+    long long rows = ((N + pieces - 1) / pieces + 255) / 256 * 256;
+    if (rows * row > W_COPY) rows = W_COPY / row / 256 * 256;        // (at least 256: rows are at most 128 KiB)
     if (rows < N) q.piece = static_cast<int>(rows);
   }
   q.tail_rows = N % q.piece;

@@ -186,3 +186,16 @@ def test_rows_that_an_int_does_not_hold_are_refused():
     one = torch.ones(1, device="cuda")
     with pytest.raises(ctypes.ArgumentError, match="does not fit"):
         L.int8_matmul(q, one, q, one)
+
+
+def test_weights_are_copied_48_mib_at_a_time_at_most():
+    """Also where a piece's rows, rounded up to tiles, would be more."""
+    lib = _lib.lib()
+    for k in (17, 577, 4099, 14337, 60001, 131071):
+        row = (k + 15) // 16 * 16
+        for n in (3000, 385, 1000, 5003, 20000, 300000):
+            counters = lib.lcq_int8_matmul_workspace_bytes(16, 1, 1, 1, 0) - 1024
+            copied = lib.lcq_int8_matmul_workspace_bytes(16, n, k, 1, 0) - counters
+            assert copied <= 48 << 20 and copied >= min(n * row, 24 << 20), (n, k, copied)
+            p = plan(16, n, k, aligned=0)
+            assert p["piece"] == n or p["piece"] % 256 == 0
