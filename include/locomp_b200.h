@@ -186,7 +186,7 @@ int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
  *   before the kernel ahead on the stream has completed: unlike lcq_matmul_int4, weights may be written by it.
  *
  * lcq_quantize_tokens: q[r, :] = rint(v / s), scales[r] = s = max|v| / 127 with v = x[r, :] or, where `weight` is given,
- *   rms_norm(x[r, :]) as in lcq_rms_norm.  A row of zeros has s = 1; s is at least 2^-126; a row that holds an infinity or a NaN gets
+ *   rms_norm(x[r, :]) as in lcq_rms_norm.  A row of zeros has s = 1 (one of no values is refused); s is at least 2^-126; a row that holds an infinity or a NaN gets
  *   s = NaN and q = 0, so that every product with it is NaN.  Without `weight` the other rows' results are those of lcq_quantize_int8 (style 0, group_size = n).
  *   x of `dtype`, rows ldx elements apart; q int8, rows ldq bytes apart (multiples of 16 suit lcq_int8_matmul); scales float32 [rows].
  * lcq_silu_mul_tokens: the same of v = gate * sigmoid(gate) * up; gate and up may be halves of the rows of one matrix.

@@ -827,8 +827,9 @@ int lcq_int8_matmul_plan_check(int M, int N, int K, int sm_count, int w_on_16, i
   return check_int8_tiling(q.main, M, q.piece, K, sm_count);
 }
 
-static int check_rows(const char* what, int64_t rows, int n, int dtype) {
+static int check_rows(const char* what, int64_t rows, int n, int dtype, bool quantized) {
   if (rows < 0 || n < 0) { set_error("%s: negative size", what); return LCQ_ERR_BAD_ARG; }
+  if (quantized && rows > 0 && n == 0) { set_error("%s: rows of no values have no scale", what); return LCQ_ERR_BAD_ARG; }
   if (!dtype_ok(dtype)) { set_error("%s: bad dtype code %d", what, dtype); return LCQ_ERR_BAD_ARG; }
   if (n > (1 << 30)) { set_error("%s: rows of %d values are not supported", what, n); return LCQ_ERR_UNSUPPORTED; }
   return LCQ_OK;
@@ -836,9 +837,9 @@ static int check_rows(const char* what, int64_t rows, int n, int dtype) {
 
 int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q, int64_t ldq, void* scales, int64_t rows, int n, float eps,
                         int dtype, void* stream) {
-  int rc = check_rows("quantize_tokens", rows, n, dtype);
+  int rc = check_rows("quantize_tokens", rows, n, dtype, true);
   if (rc != LCQ_OK) return rc;
-  if (rows == 0 || n == 0) return LCQ_OK;
+  if (rows == 0) return LCQ_OK;
   if (!x || !q || !scales) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
   if (rows > 1 && (ldx < n || ldq < n)) { set_error("quantize_tokens: rows must be at least n=%d apart", n); return LCQ_ERR_BAD_ARG; }
   rows::Args a = {};
@@ -857,9 +858,9 @@ int lcq_quantize_tokens(const void* x, int64_t ldx, const void* weight, void* q,
 
 int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, void* q, int64_t ldq, void* scales, int64_t rows,
                         int n, int dtype, void* stream) {
-  int rc = check_rows("silu_mul_tokens", rows, n, dtype);
+  int rc = check_rows("silu_mul_tokens", rows, n, dtype, true);
   if (rc != LCQ_OK) return rc;
-  if (rows == 0 || n == 0) return LCQ_OK;
+  if (rows == 0) return LCQ_OK;
   if (!gate || !up || !q || !scales) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
   if (rows > 1 && (ld_gate < n || ld_up < n || ldq < n)) { set_error("silu_mul_tokens: rows must be at least n=%d apart", n); return LCQ_ERR_BAD_ARG; }
   rows::Args a = {};
@@ -878,7 +879,7 @@ int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64
 int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
                        const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n, float eps, int dtype,
                        void* stream) {
-  int rc = check_rows("residual_norms", rows, n, dtype);
+  int rc = check_rows("residual_norms", rows, n, dtype, scales != nullptr);
   if (rc != LCQ_OK) return rc;
   if (rows == 0 || n == 0) return LCQ_OK;
   if (!hidden || !delta || !hidden_out || (weight && !out)) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }

@@ -77,13 +77,15 @@ def _empty_tokens(shape, device) -> QuantizedTokens:
 
 def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[QuantizedTokens, int, int, int]:
     """The tokens a call writes, the addresses of q and scales, and how far apart the rows of q are."""
+    rows, n = 1, shape[-1]
+    for size in shape[:-1]:
+        rows *= size
+    if rows and not n:
+        raise ValueError("rows of no values have no scale")
     if out is None:
         out = _empty_tokens(shape, torch.device("cuda", dev))
     elif not isinstance(out, QuantizedTokens):
         raise TypeError(f"out must be QuantizedTokens, got {type(out)}")
-    rows, n = 1, shape[-1]
-    for size in shape[:-1]:
-        rows *= size
     qo, ld = _resolve_rows(out.q, "out.q")
     so = resolve(out.scales, "out.scales")
     if qo.kind != "i8" or qo.size != rows * n or (rows and qo.shape[-1] != n):

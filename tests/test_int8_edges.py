@@ -172,7 +172,7 @@ def test_sizes_that_an_int_does_not_hold_are_refused():
     for call in calls:
         with pytest.raises(ctypes.ArgumentError, match="does not fit"):
             call()
-    assert lib.lcq_quantize_tokens(None, 0, None, None, 0, None, big, 0, 1e-5, 0, None) == 0          # rows are 64 bits
+    assert lib.lcq_residual_norms(None, None, None, None, 0, 1.0, None, None, None, 0, None, big, 0, 1e-5, 0, None) == 0      # rows are 64 bits
 
 
 @pytest.mark.gpu
@@ -199,3 +199,34 @@ def test_weights_are_copied_48_mib_at_a_time_at_most():
             assert copied <= 48 << 20 and copied >= min(n * row, 24 << 20), (n, k, copied)
             p = plan(16, n, k, aligned=0)
             assert p["piece"] == n or p["piece"] % 256 == 0
+
+
+def test_rows_of_no_values_have_no_scale():
+    """They used to return with their scales left as they were."""
+    lib, p, bad = _lib.lib(), ctypes.c_void_p(4096), _lib.ERR_BAD_ARG
+    assert lib.lcq_quantize_tokens(p, 0, None, p, 0, p, 5, 0, 1e-5, 0, None) == bad
+    assert lib.lcq_silu_mul_tokens(p, 0, p, 0, p, 0, p, 5, 0, 0, None) == bad
+    assert lib.lcq_residual_norms(p, p, None, None, 0, 1.0, p, p, p, 0, p, 5, 0, 1e-5, 0, None) == bad
+    assert lib.lcq_residual_norms(p, p, None, None, 0, 1.0, p, p, p, 0, None, 5, 0, 1e-5, 0, None) == 0
+    for rows in (0, 5):
+        assert lib.lcq_quantize_tokens(p, 8, None, p, 8, p, 0, rows, 1e-5, 0, None) == 0
+
+
+@pytest.mark.gpu
+def test_calls_on_nothing():
+    for kind in KINDS:
+        for shape in ((5, 0), (2, 3, 0), (0,)):
+            x = torch.empty(shape, device="cuda", dtype=kind)
+            for call in (lambda: L.quantize_tokens(x), lambda: L.silu_mul_tokens(x, x), lambda: L.quantize_tokens(x, x.reshape(-1)[:0]),
+                         lambda: L.residual_norms(x, x, torch.empty(0, device="cuda", dtype=kind), quantized=True)):
+                with pytest.raises(ValueError, match="no scale"):
+                    call()
+            assert L.residual_norms(x, x) is x
+        none = torch.empty(0, 64, device="cuda", dtype=kind)
+        w = torch.ones(64, device="cuda", dtype=kind)
+        for t in (L.quantize_tokens(none, w), L.silu_mul_tokens(none, none), L.residual_norms(none, none, w, quantized=True)):
+            assert t.q.shape == (0, 64) and t.scales.shape == (0,)
+        assert L.residual_norms(none, none, w).shape == (0, 64)
+        one = torch.ones(3, device="cuda")
+        with pytest.raises(ValueError, match="K=0"):
+            L.int8_matmul(torch.empty(3, 0, dtype=torch.int8, device="cuda"), one, torch.empty(3, 0, dtype=torch.int8, device="cuda"), one)
