@@ -69,6 +69,15 @@ def _rows_of(op: Operand, name: str) -> Tuple[int, int]:
     return (op.size // n if n else 0), n
 
 
+def _pair(out):
+    """The tensors of the tokens that a call is given to write."""
+    if out is None:
+        return None
+    if not isinstance(out, QuantizedTokens):
+        raise TypeError(f"out must be QuantizedTokens, got {type(out)}")
+    return out.q, out.scales
+
+
 def _empty_tokens(shape, device) -> QuantizedTokens:
     n = shape[-1]
     wide = torch.empty(tuple(shape[:-1]) + ((n + 15) // 16 * 16,), dtype=torch.int8, device=device)
@@ -82,12 +91,12 @@ def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[Quanti
         rows *= size
     if rows and not n:
         raise ValueError("rows of no values have no scale")
-    if out is None:
+    given = _pair(out)
+    if given is None:
         out = _empty_tokens(shape, torch.device("cuda", dev))
-    elif not isinstance(out, QuantizedTokens):
-        raise TypeError(f"out must be QuantizedTokens, got {type(out)}")
-    qo, ld = _resolve_rows(out.q, "out.q")
-    so = resolve(out.scales, "out.scales")
+        given = _pair(out)
+    qo, ld = _resolve_rows(given[0], "out.q")
+    so = resolve(given[1], "out.scales")
     if qo.kind != "i8" or qo.size != rows * n or (rows and qo.shape[-1] != n):
         raise ValueError(f"out.q must hold {rows} int8 rows of {n}")
     if so.kind != "f32" or so.size != rows:
@@ -107,7 +116,7 @@ def quantize_tokens(x, weight=None, eps: float = 1e-5, *, out: Optional[Quantize
     has scale NaN (and q 0), and so do all products with it.  Without `weight`: the values and scales of quantize(x, n, bits=8), but for
     such rows and for scales that would be below 2**-126."""
     if stream is None and not bf16 and isinstance(x, torch.Tensor):
-        res = _lib.calls.quantize_tokens(x, weight, eps, None if out is None else (out.q, out.scales))
+        res = _lib.calls.quantize_tokens(x, weight, eps, _pair(out))
         if res is not NotImplemented:
             return QuantizedTokens(*res) if out is None else out
     xo, ldx = _resolve_rows(x, "x", bf16)
@@ -129,7 +138,7 @@ def silu_mul_tokens(gate, up, *, out: Optional[QuantizedTokens] = None, stream=N
     """gate * sigmoid(gate) * up as int8 tokens (see quantize_tokens).  gate and up: [n] or [rows, n]; they may be the halves
     gu[:, :n] and gu[:, n:] of what a fused projection gave."""
     if stream is None and not bf16 and isinstance(gate, torch.Tensor):
-        res = _lib.calls.silu_mul_tokens(gate, up, None if out is None else (out.q, out.scales))
+        res = _lib.calls.silu_mul_tokens(gate, up, _pair(out))
         if res is not NotImplemented:
             return QuantizedTokens(*res) if out is None else out
     (go, ldg), (uo, ldu) = _resolve_rows(gate, "gate", bf16), _resolve_rows(up, "up", bf16)

@@ -230,3 +230,12 @@ def test_calls_on_nothing():
         one = torch.ones(3, device="cuda")
         with pytest.raises(ValueError, match="K=0"):
             L.int8_matmul(torch.empty(3, 0, dtype=torch.int8, device="cuda"), one, torch.empty(3, 0, dtype=torch.int8, device="cuda"), one)
+
+
+# ------------------------------------------------------------------------------------------ outputs and layers
+def test_tokens_go_into_tokens():
+    x = torch.zeros(4, 64)
+    for call in (lambda out: L.quantize_tokens(x, out=out), lambda out: L.silu_mul_tokens(x, x, out=out)):
+        for out in (torch.zeros(4, 64, dtype=torch.int8), (x, x), 3):
+            with pytest.raises(TypeError, match="QuantizedTokens"):
+                call(out)
