@@ -475,10 +475,9 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   long long wanted;
   if (!x || !xs || !w || !ws || !as_int(args[5], wanted) || wanted < -1 || wanted > LCQ_BF16) return not_implemented();
   if (x->scalar_type() != at::kChar || w->scalar_type() != at::kChar || xs->scalar_type() != at::kFloat) return not_implemented();
-  const bool row = x->dim() == 1;
-  if ((!row && x->dim() != 2) || w->dim() != 2 || w->device() != x->device() || xs->device() != x->device() || ws->device() != x->device())
+  if ((x->dim() > 2 && xs->sizes() != x->sizes().slice(0, x->dim() - 1)) || w->dim() != 2 || w->device() != x->device() || xs->device() != x->device() || ws->device() != x->device())
     return not_implemented();
-  const int64_t M = row ? 1 : x->size(0), K = x->size(-1), N = w->size(0);
+  const int64_t K = x->size(-1), M = x->numel() / K, N = w->size(0);
   constexpr int64_t most = 2000000000;
   const int sk = float_code(ws->scalar_type());
   if (w->size(1) != K || xs->numel() != M || ws->numel() != N || sk == NOT_FLOAT || M > most || N > most || K > most) return not_implemented();
@@ -487,7 +486,9 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   int ok = wanted < 0 ? LCQ_F16 : static_cast<int>(wanted);
   const c10::cuda::OptionalCUDAGuard guard(x->device());
   if (args[4] == Py_None) {
-    made = row ? empty({N}, float_type(ok), *x) : empty({M, N}, float_type(ok), *x);
+    c10::SmallVector<int64_t, 6> shape(x->sizes().begin(), x->sizes().end());
+    shape.back() = N;
+    made = empty(shape, float_type(ok), *x);
   } else {
     out = cuda_tensor(args[4]);
     if (!out || out->device() != x->device() || out->numel() != M * N) return not_implemented();

@@ -111,7 +111,7 @@ def _tokens_out(out: Optional[QuantizedTokens], shape, dev: int) -> Tuple[Quanti
 # ------------------------------------------------------------------------------------------ rows
 def quantize_tokens(x, weight=None, eps: float = 1e-5, *, out: Optional[QuantizedTokens] = None, stream=None,
                     bf16: bool = False) -> QuantizedTokens:
-    """x ([n] or [rows, n]; rows may be further apart than n) as int8 tokens: scale = max|v| / 127 over a row, q = rint(v / scale),
+    """x ([n], [rows, n] or [..., n]; rows may be further apart than n) as int8 tokens: scale = max|v| / 127 over a row, q = rint(v / scale),
     with v = x or, where `weight` is given, rms_norm(x, weight, eps).  A row of zeros has scale 1; a row that holds an infinity or a NaN
     has scale NaN (and q 0), and so do all products with it.  Without `weight`: the values and scales of quantize(x, n, bits=8), but for
     such rows and for scales that would be below 2**-126."""
@@ -225,9 +225,10 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
                 workspace_buf: Optional[torch.Tensor] = None):
     """out[m, n] = (sum_k x[m, k] * w[n, k]) * x_scales[m] * w_scales[n]: an exact integer sum, scaled in float32 and rounded once.
 
-    x: int8 [K] or [M, K]; x_scales: float32, M values; w: int8 [N, K]; w_scales: N values (f32 / f16 / bf16).  Rows of x and w may be
+    x: int8 [K] or [M, K]; x_scales: float32, M values; w: int8 [N, K]; w_scales: N values (f32 / f16 / bf16).  x may have more dimensions, as
+    quantize_tokens gives them for a batch of sequences: [..., K] with x_scales of the shape [...].  Rows of x and w may be
     further apart than K; those that do not start on 16 bytes (K % 16 != 0 in contiguous storage) cost a copy.
-    Returns a torch CUDA tensor [N] or [M, N] of out_dtype ("f32", "f16", "bf16"; default "f16") or `out`.  K is at most 131071.
+    Returns a torch CUDA tensor [N], [M, N] or [..., N] of out_dtype ("f32", "f16", "bf16"; default "f16") or `out`.  K is at most 131071.
     Scratch is needed for such copies only: workspace_buf, or this package's buffer of the stream; under CUDA-graph capture the graph's own memory,
     so that no two graphs share it."""
     if isinstance(x, torch.Tensor) and stream is None:
@@ -239,12 +240,13 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
     for op, name in ((xo, "x"), (wo, "w")):
         if op.kind != "i8":
             raise TypeError(f"{name} must be int8, got {op.kind}")
-    if len(xo.shape) not in (1, 2):
-        raise ValueError(f"x must be [K] or [M, K], got shape {xo.shape}")
+    if not xo.shape or (len(xo.shape) > 2 and xso.shape != xo.shape[:-1]):
+        raise ValueError(f"x must be [K] or [M, K], or [..., K] with x_scales of [...], got shapes {xo.shape} and {xso.shape}")
     if len(wo.shape) != 2:
         raise ValueError(f"w must be [N, K], got shape {wo.shape}")
-    squeeze = len(xo.shape) == 1
-    M, K, N = 1 if squeeze else xo.shape[0], xo.shape[-1], wo.shape[0]
+    M, K, N = 1, xo.shape[-1], wo.shape[0]
+    for size in xo.shape[:-1]:
+        M *= size
     if wo.shape[1] != K:
         raise ValueError(f"x has K={K} but the weights hold K={wo.shape[1]}")
     if xso.kind != "f32" or xso.size != M:
@@ -258,7 +260,7 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
     _require_cuda()
     L = _lib.lib()
     with _on(dev, stream):
-        res = torch.empty((M, N), dtype=KIND_TO_TORCH[out_dtype or "f16"], device=torch.device("cuda", dev)) if out is None else out
+        res = torch.empty(xo.shape[:-1] + (N,), dtype=KIND_TO_TORCH[out_dtype or "f16"], device=torch.device("cuda", dev)) if out is None else out
         oo = resolve(res, "out")
         if oo.size != M * N:
             raise ValueError(f"out must hold M*N = {M * N} values, got {oo.size}")
@@ -288,7 +290,7 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
                 launch(workspace(need, dev, sp))
         if oo.host is not None:
             return _finish(oo, res)
-    return res[0] if out is None and squeeze else res
+    return res
 
 
 def _on_16(op: Operand, rows: int, ld: int) -> bool:
@@ -308,7 +310,7 @@ class Int8Linear:
     """y = x @ (w * scales)^T in int8: w int8 [N, K] and one scale for each of its rows, as quantize(weights, K, bits=8) makes them.
 
     linear(x): x is QuantizedTokens, or float activations, which are quantised first; linear(x, weight): their RMS norm with that
-    weight is.  The result has the type of the activations (tokens: float16), or out_dtype, or is written to `out`."""
+    weight is.  x: [K], [M, K] or [..., K].  The result has the type of the activations (tokens: float16), or out_dtype, or is written to `out`."""
 
     def __init__(self, w: torch.Tensor, scales: torch.Tensor):
         if not (w.is_cuda and scales.is_cuda):

@@ -239,3 +239,40 @@ def test_tokens_go_into_tokens():
         for out in (torch.zeros(4, 64, dtype=torch.int8), (x, x), 3):
             with pytest.raises(TypeError, match="QuantizedTokens"):
                 call(out)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,n,k", [((2, 3), 40, 100), ((1, 1), 40, 64), ((4, 1, 5), 300, 512), ((2, 150), 256, 333), ((8, 1), 64, 96)])
+def test_batches_of_sequences(shape, n, k):
+    """Tokens of more dimensions go through the product and the layer as their rows do."""
+    g = gen(n, k)
+    q = L.quantize(torch.randn(n, k, device="cuda", generator=g), k, bits=8)
+    layer, w = q.int8_linear(), 1 + 0.1 * torch.randn(k, device="cuda", generator=g)
+    x = torch.randn(*shape, k, device="cuda", generator=g)
+    rows = x.numel() // k
+    t = L.quantize_tokens(x)
+    y = L.int8_matmul(t.q, t.scales, q.w, q.scales, out_dtype="f32")
+    flat = L.quantize_tokens(x.view(rows, k))
+    want = L.int8_matmul(flat.q, flat.scales, q.w, q.scales, out_dtype="f32")
+    assert y.shape == shape + (n,) and torch.equal(y.view(rows, n), want)
+    check_product(y.view(rows, n), flat.q.double() @ q.w.double().t() * flat.scales.double()[:, None] * q.scales.double().view(-1), torch.float32)
+    assert torch.equal(layer(x), y) and torch.equal(layer(t, out_dtype="f32"), y)
+    assert torch.equal(layer(x, w).view(rows, n), layer(x.view(rows, k), w))
+    D = L.DeviceTensor                                       # the general path
+    assert torch.equal(L.int8_matmul(D(t.q.contiguous()), t.scales, q.w, q.scales, out_dtype="f32"), y)
+    out = torch.empty(shape + (n,), device="cuda")
+    assert layer(x, out=out) is out and torch.equal(out, y)
+    out = torch.empty(rows, n, device="cuda")
+    assert L.int8_matmul(t.q, t.scales, q.w, q.scales, out=out) is out and torch.equal(out, want)
+    wide = torch.randint(-128, 128, shape + (k + 16,), dtype=torch.int8, device="cuda", generator=g)[..., 5:5 + k]
+    assert torch.equal(L.int8_matmul(wide, t.scales, q.w, q.scales, out_dtype="f32"),
+                       L.int8_matmul(wide.contiguous(), t.scales, q.w, q.scales, out_dtype="f32"))
+    for scales in (t.scales.reshape(-1), t.scales[None]):
+        with pytest.raises(ValueError, match="must be \\[K\\]"):
+            L.int8_matmul(t.q, scales, q.w, q.scales)
+    with pytest.raises(ValueError, match="contiguous"):
+        L.int8_matmul(t.q[:, :1].expand(t.q.shape) if shape[1] > 1 else t.q[:1].expand((3,) + t.q.shape[1:]),
+                      t.scales if shape[1] > 1 else torch.ones((3,) + t.scales.shape[1:], device="cuda"), q.w, q.scales)
+    empty = L.quantize_tokens(x[:0])
+    assert layer(empty).shape == (0,) + shape[1:] + (n,)
+    status_ok()
