@@ -320,7 +320,7 @@ class Int8Linear:
         if scales.numel() != w.shape[0]:
             raise ValueError(f"scales must hold N = {w.shape[0]} values, got {scales.numel()}")
         self.out_features, self.in_features = w.shape
-        if w.stride(1) != 1 or w.stride(0) % 16 or w.data_ptr() % 16:          # rows on 16 bytes, for TMA
+        if w.stride(1) != 1 or w.stride(0) < self.in_features or w.stride(0) % 16 or w.data_ptr() % 16:      # rows on 16 bytes, for TMA
             wide = torch.zeros(self.out_features, (self.in_features + 15) // 16 * 16, dtype=torch.int8, device=w.device)
             wide[:, :self.in_features] = w
             w = wide[:, :self.in_features]

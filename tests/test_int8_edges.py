@@ -276,3 +276,16 @@ def test_batches_of_sequences(shape, n, k):
     empty = L.quantize_tokens(x[:0])
     assert layer(empty).shape == (0,) + shape[1:] + (n,)
     status_ok()
+
+
+@pytest.mark.gpu
+def test_a_layer_of_weights_whose_rows_lie_on_one_another():
+    """A broadcast weight is copied, as every other whose rows the product cannot read in place; it was kept, and every call refused it."""
+    g = gen(3)
+    row = torch.randint(-127, 128, (1, 64), dtype=torch.int8, device="cuda", generator=g)
+    scales, x = torch.rand(24, device="cuda", generator=g), torch.randn(5, 64, device="cuda", generator=g)
+    for w in (row.expand(24, 64), torch.randint(-127, 128, (48 + 23 * 16,), dtype=torch.int8, device="cuda", generator=g).as_strided((24, 48), (16, 1)),
+              torch.randint(-127, 128, (64, 24), dtype=torch.int8, device="cuda", generator=g).t()):
+        k = w.shape[1]
+        assert torch.equal(L.Int8Linear(w, scales)(x[:, :k].contiguous()), L.Int8Linear(w.contiguous(), scales)(x[:, :k].contiguous()))
+    status_ok()
