@@ -195,6 +195,8 @@ int lcq_add_inplace(void* a, const void* b, int64_t n, int dtype, void* stream);
  *     out = rms_norm(hidden_out) * weight, of `dtype`, or (scales given) as int8 tokens.
  *   post_weight and gate may be NULL; weight NULL: no norm follows, out is not written.  gate: [gate_rows, n], rows % gate_rows == 0.
  *   hidden, delta, hidden_out [rows, n], contiguous; hidden_out may be hidden, and out (not int8) may be delta.
+ * lcq_residual_norms_delta: the same with a type of delta's own, `dtype` or LCQ_F32 (out is not delta then): what a product leaves in float32 is rounded once, as it is
+ *   added.
  */
 int lcq_int8_matmul(const void* x, int64_t ldx, const void* x_scales, const void* w, int64_t ldw, const void* w_scales, void* out,
                     int M, int N, int K, int w_scale_dtype, int out_dtype, void* workspace, size_t workspace_bytes, void* stream);
@@ -206,6 +208,9 @@ int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64
 int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
                        const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n, float eps,
                        int dtype, void* stream);
+int lcq_residual_norms_delta(const void* hidden, const void* delta, int delta_dtype, const void* post_weight, const void* gate, int64_t gate_rows,
+                             float scale, const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n,
+                             float eps, int dtype, void* stream);
 
 /*
  * Embedding lookup: out[t, :] = table[token_ids[t], :]; token_ids int32 [tokens], table [vocab, dim],

@@ -66,6 +66,8 @@ SIGNATURES = {
                                        _c.c_int, _c.c_int, _c.c_void_p]),
     "lcq_residual_norms": (_c.c_int, [_c.c_void_p] * 4 + [_c.c_int64, _c.c_float] + [_c.c_void_p] * 3 + [_c.c_int64, _c.c_void_p, _c.c_int64,
                                       _c.c_int, _c.c_float, _c.c_int, _c.c_void_p]),
+    "lcq_residual_norms_delta": (_c.c_int, [_c.c_void_p] * 2 + [_c.c_int] + [_c.c_void_p] * 2 + [_c.c_int64, _c.c_float] + [_c.c_void_p] * 3 +
+                                 [_c.c_int64, _c.c_void_p, _c.c_int64, _c.c_int, _c.c_float, _c.c_int, _c.c_void_p]),
     "lcq_embed_lookup": (_c.c_int, [_c.c_void_p] * 3 + [_c.c_int64, _c.c_int, _c.c_int, _c.c_int, _c.c_void_p]),
     "lcq_argmax": (_c.c_int, [_c.c_void_p] * 2 + [_c.c_int64, _c.c_int, _c.c_int, _c.c_void_p]),
     "lcq_decode_step_state_bytes": (_c.c_size_t, [_c.POINTER(DecodeStackDesc)]),

@@ -879,8 +879,16 @@ int lcq_silu_mul_tokens(const void* gate, int64_t ld_gate, const void* up, int64
 int lcq_residual_norms(const void* hidden, const void* delta, const void* post_weight, const void* gate, int64_t gate_rows, float scale,
                        const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n, float eps, int dtype,
                        void* stream) {
+  return lcq_residual_norms_delta(hidden, delta, dtype, post_weight, gate, gate_rows, scale, weight, hidden_out, out, ld_out, scales, rows, n, eps, dtype,
+                                  stream);
+}
+
+int lcq_residual_norms_delta(const void* hidden, const void* delta, int delta_dtype, const void* post_weight, const void* gate, int64_t gate_rows,
+                             float scale, const void* weight, void* hidden_out, void* out, int64_t ld_out, void* scales, int64_t rows, int n,
+                             float eps, int dtype, void* stream) {
   int rc = check_rows("residual_norms", rows, n, dtype, scales != nullptr);
   if (rc != LCQ_OK) return rc;
+  if (delta_dtype != dtype && delta_dtype != LCQ_F32) { set_error("residual_norms: delta is of hidden's type or float32, not of code %d", delta_dtype); return LCQ_ERR_BAD_ARG; }
   if (rows == 0 || n == 0) return LCQ_OK;
   if (!hidden || !delta || !hidden_out || (weight && !out)) { set_error("null pointer argument"); return LCQ_ERR_BAD_ARG; }
   if (scales && !weight) { set_error("residual_norms: int8 tokens are those of the norm, which needs a weight"); return LCQ_ERR_BAD_ARG; }
@@ -902,6 +910,12 @@ int lcq_residual_norms(const void* hidden, const void* delta, const void* post_w
   rc = current_dev_info(di);
   if (rc != LCQ_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (delta_dtype != dtype) {
+    if (dtype == LCQ_F16)
+      return scales ? rows::launch<__half, rows::RESIDUAL, true, float>(a, di.sm_count, st) : rows::launch<__half, rows::RESIDUAL, false, float>(a, di.sm_count, st);
+    return scales ? rows::launch<__nv_bfloat16, rows::RESIDUAL, true, float>(a, di.sm_count, st)
+                  : rows::launch<__nv_bfloat16, rows::RESIDUAL, false, float>(a, di.sm_count, st);
+  }
   if (scales) { LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, true>(a, di.sm_count, st))) }
   LCQ_BY_DTYPE(dtype, (rows::launch<T, rows::RESIDUAL, false>(a, di.sm_count, st)))
 }

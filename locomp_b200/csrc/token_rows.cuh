@@ -8,6 +8,7 @@
 // and v goes out in the storage type (RESIDUAL), or as int8 with a float32 scale for the row:
 //   s = max |v| / 127 (at least 2^-126; 1 for a row of zeros), q = rint(v / s).
 // A row that holds an infinity or NaN gets the scale NaN and q = 0, so that every product with it is NaN, and no other row's.
+// delta may be float32 where hidden is 16 bits wide: a product's result that is normalised and added here need not be rounded between.
 // All arithmetic is float32.  Without a norm s and q are bit for bit those of the weight quantiser with the row as its group.
 // With one, the factor rsqrt(..) is common to v and s: q is taken from the products with the weight alone, and one reduction finds
 // their maximum together with the sum of squares.
@@ -241,10 +242,11 @@ __device__ __forceinline__ void store_q(int8_t* row, int i, int n, const float (
 }
 
 // E octets a thread; WARP_ROW: four rows a block, a warp each; WHOLE: a row fits into the registers of its threads.
-template <typename T, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
+// D: the type of b (T, or of RESIDUAL's delta also float).
+template <typename T, typename D, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
 __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p) {
   using Rw = Raw<T, ALIGNED>;
-  constexpr bool PAIRS = ALIGNED || sizeof(T) == 2;
+  constexpr bool PAIRS = ALIGNED || sizeof(D) == 2;
   __shared__ float2 red[2][32];
   griddep_launch_dependents();
   griddep_wait();
@@ -253,7 +255,7 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
   const int n = p.n;
   const int t = WARP_ROW ? threadIdx.x & 31 : threadIdx.x, per_octet = 8 * (WARP_ROW ? 32 : blockDim.x), per_chunk = E * per_octet;
   const T* a = static_cast<const T*>(p.a) + row * p.lda;
-  const T* b = static_cast<const T*>(p.b) + row * p.ldb;
+  const D* b = static_cast<const D*>(p.b) + row * p.ldb;
   const T* weight = static_cast<const T*>(p.weight);
   const T* post = static_cast<const T*>(p.post_weight);
   const T* gate = static_cast<const T*>(p.gate);
@@ -270,10 +272,12 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
     w.octet(src, i, n).get(f);
   };
 
-  Octet<T> x[E], y[E];                               // RESIDUAL: hidden, delta
+  Octet<T> x[E];                                     // RESIDUAL: hidden
+  Octet<D> y[E];                                     // delta
   // all loads of a chunk on their way, then the values
-  const auto fetch = [&](const T* src_x, const T* src_y, int c0) {
-    Rw rx[E], ry[E];
+  const auto fetch = [&](const T* src_x, const D* src_y, int c0) {
+    Rw rx[E];
+    Raw<D, ALIGNED> ry[E];
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int i = i0 + c0 + e * per_octet;
@@ -411,14 +415,14 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
 }
 
 // ---------------------------------------------------------------------------- host side
-template <typename T, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
+template <typename T, typename D, int OP, bool QUANT, bool ALIGNED, int E, bool WARP_ROW, bool WHOLE, int MAX_THREADS, int BLOCKS>
 int launch_form(const Args& p, int threads, cudaStream_t st) {
   const long long blocks = WARP_ROW ? (p.n_rows + 3) / 4 : p.n_rows;
   if (blocks > 2147483647LL) { set_error("more than 2^31 rows"); return LCQ_ERR_UNSUPPORTED; }
   cudaLaunchConfig_t cfg;
   cudaLaunchAttribute attr[1];
   glue::pdl_config(cfg, attr, dim3(static_cast<unsigned>(blocks)), dim3(threads), st);
-  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<T, OP, QUANT, ALIGNED, E, WARP_ROW, WHOLE, MAX_THREADS, BLOCKS>, p));
+  LCQ_CUDA_TRY(cudaLaunchKernelEx(&cfg, rows_kernel<T, D, OP, QUANT, ALIGNED, E, WARP_ROW, WHOLE, MAX_THREADS, BLOCKS>, p));
   return LCQ_OK;
 }
 // The forms and where each is the faster (us, B200; n values a row, E octets a thread).
@@ -426,44 +430,46 @@ int launch_form(const Args& p, int threads, cudaStream_t st) {
 //   E = 1, most threads a row         few rows, where latency counts (1 x 4096: 2.6; E = 2 3.2, E = 4 4.4), and RESIDUAL up to 2048 values or 8 Mi in all
 //   E = 4, most bytes on their way    all other 16-bit rows up to 16,384 (8192 x 8192 RESIDUAL: 87; E = 1 122, E = 2 98, E = 8 101)
 //   E = 2                             float32, and rows off 16 bytes, which hold more registers for each octet (4000 x 5003: 48; E = 1 59, E = 4 56)
+//                                     (a float32 delta beside 16 bits counts as float32: 1000 x 2048 4.6 for 4.2 with 16 bits, 8192 x 8192 107 for 81, both at
+//                                     the copy rate)
 //   E = 8                             16-bit rows up to 32,768 of one operand (4000 x 28,672 quantised: 69; E = 4 93); of two, E = 4 in twice the threads
 //                                     (1000 x 28,672 SILU_MUL: 39; E = 8 44, in chunks 58)
-template <typename T, int OP, bool QUANT, bool ALIGNED>
+template <typename T, typename D, int OP, bool QUANT, bool ALIGNED>
 int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
-  constexpr bool HALF = sizeof(T) == 2, ONE = OP == ROWS || OP == NORM_ROWS;
+  constexpr bool HALF = sizeof(D) == 2, ONE = OP == ROWS || OP == NORM_ROWS;
   const int span = p.n + (ALIGNED ? 0 : 7);          // (an octet may begin up to seven values before the row)
   const auto threads = [&](int e) { return ((span + 8 * e - 1) / (8 * e) + 31) / 32 * 32; };
   const bool few = p.n_rows <= 2ll * sm_count;
-  if (span <= 512 && p.n_rows >= 4) return launch_form<T, OP, QUANT, ALIGNED, 2, true, true, 128, 8>(p, 128, st);
+  if (span <= 512 && p.n_rows >= 4) return launch_form<T, D, OP, QUANT, ALIGNED, 2, true, true, 128, 8>(p, 128, st);
   if constexpr (ONE) {
-    if (span <= 1024 && !few) return launch_form<T, OP, QUANT, ALIGNED, 4, true, true, 128, 4>(p, 128, st);
+    if (span <= 1024 && !few) return launch_form<T, D, OP, QUANT, ALIGNED, 4, true, true, 128, 4>(p, 128, st);
   }
   if (span <= 8192 && (few || (HALF && ALIGNED && OP == RESIDUAL && (p.n <= 2048 || p.n_rows * p.n <= (8ll << 20)))))
-    return launch_form<T, OP, QUANT, ALIGNED, 1, false, true, 1024, 2>(p, threads(1), st);
+    return launch_form<T, D, OP, QUANT, ALIGNED, 1, false, true, 1024, 2>(p, threads(1), st);
   if constexpr (!HALF || !ALIGNED) {
-    if (span <= 8192) return launch_form<T, OP, QUANT, ALIGNED, 2, false, true, 512, 2>(p, threads(2), st);
-    if (span <= 16384) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 512, 1>(p, threads(4), st);
+    if (span <= 8192) return launch_form<T, D, OP, QUANT, ALIGNED, 2, false, true, 512, 2>(p, threads(2), st);
+    if (span <= 16384) return launch_form<T, D, OP, QUANT, ALIGNED, 4, false, true, 512, 1>(p, threads(4), st);
   } else {
-    if (span <= 16384) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 512, ONE ? 3 : 2>(p, threads(4), st);
+    if (span <= 16384) return launch_form<T, D, OP, QUANT, ALIGNED, 4, false, true, 512, ONE ? 3 : 2>(p, threads(4), st);
   }
   if constexpr (HALF) {
     if constexpr (ONE) {
-      if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 8, false, true, 512, 2>(p, threads(8), st);
+      if (span <= 32768) return launch_form<T, D, OP, QUANT, ALIGNED, 8, false, true, 512, 2>(p, threads(8), st);
     } else {
-      if (span <= 32768) return launch_form<T, OP, QUANT, ALIGNED, 4, false, true, 1024, 1>(p, threads(4), st);
+      if (span <= 32768) return launch_form<T, D, OP, QUANT, ALIGNED, 4, false, true, 1024, 1>(p, threads(4), st);
     }
   }
-  return launch_form<T, OP, QUANT, ALIGNED, 2, false, false, 512, 2>(p, 512, st);
+  return launch_form<T, D, OP, QUANT, ALIGNED, 2, false, false, 512, 2>(p, 512, st);
 }
 
 // Octets as they lie where every row of every operand starts on 16 bytes (of q: on 8) and holds whole ones.
-template <typename T, int OP, bool QUANT>
+template <typename T, int OP, bool QUANT, typename D = T>
 int launch(const Args& p, int sm_count, cudaStream_t st) {
   const auto rows_on_16 = [&](const void* q, long long ld) { return aligned(q, 16) && (ld * sizeof(T)) % 16 == 0; };
-  const bool on_16 = p.n % 8 == 0 && rows_on_16(p.a, p.lda) && rows_on_16(p.b, p.ldb) && aligned(p.weight, 16) && aligned(p.post_weight, 16) &&
+  const bool on_16 = p.n % 8 == 0 && rows_on_16(p.a, p.lda) && aligned(p.b, 16) && (p.ldb * sizeof(D)) % 16 == 0 && aligned(p.weight, 16) && aligned(p.post_weight, 16) &&
                      aligned(p.gate, 16) && aligned(p.hidden_out, 16) &&
                      (QUANT ? aligned(p.out, 8) && p.ldo % 8 == 0 : rows_on_16(p.out, p.ldo));
-  return on_16 ? launch_aligned<T, OP, QUANT, true>(p, sm_count, st) : launch_aligned<T, OP, QUANT, false>(p, sm_count, st);
+  return on_16 ? launch_aligned<T, D, OP, QUANT, true>(p, sm_count, st) : launch_aligned<T, D, OP, QUANT, false>(p, sm_count, st);
 }
 
 }  // namespace rows

@@ -46,7 +46,7 @@ struct Api {
   decltype(&lcq_int8_matmul_workspace_bytes) int8_workspace_bytes;
   decltype(&lcq_quantize_tokens) quantize_tokens;
   decltype(&lcq_silu_mul_tokens) silu_mul_tokens;
-  decltype(&lcq_residual_norms) residual_norms;
+  decltype(&lcq_residual_norms_delta) residual_norms;
 } api;
 PyObject* raise_status = nullptr;      // callable(status): raises the exception of a negative status
 PyObject* make_workspace = nullptr;    // callable(nbytes, device, stream): allocates (or grows) and reports it through set_workspace
@@ -426,8 +426,8 @@ PyObject* residual_norms(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   if (!h || !d || h->dim() < 1 || h->numel() == 0 || !PyFloat_Check(args[3]) || !PyFloat_Check(args[6]) || !PyBool_Check(args[9]))
     return not_implemented();
   const int64_t n = h->size(-1), rows = h->numel() / n;
-  const int code = shared_code(*h, *d);
-  if (code == NOT_FLOAT || d->dim() < 1 || d->numel() != h->numel() || d->size(-1) != n || n > MOST_PER_ROW) return not_implemented();
+  const int code = float_code(h->scalar_type()), delta_code = float_code(d->scalar_type());      // (delta may be float32 beside 16 bits)
+  if (code == NOT_FLOAT || (delta_code != code && delta_code != LCQ_F32) || d->device() != h->device() || d->dim() < 1 || d->numel() != h->numel() || d->size(-1) != n || n > MOST_PER_ROW) return not_implemented();
   const at::Tensor* more[3] = {nullptr, nullptr, nullptr};        // weight, post_weight, gate
   const int where[3] = {2, 4, 5};
   for (int i = 0; i < 3; ++i) {
@@ -458,7 +458,7 @@ PyObject* residual_norms(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   const float eps = static_cast<float>(PyFloat_AS_DOUBLE(args[3])), scale = static_cast<float>(PyFloat_AS_DOUBLE(args[6]));
   const auto ptr = [](const at::Tensor* a) { return a ? a->data_ptr() : nullptr; };
   const int rc = unlocked([&] {
-    return api.residual_norms(h->data_ptr(), d->data_ptr(), ptr(more[1]), ptr(more[2]), gate_rows, scale, ptr(more[0]), ho->data_ptr(),
+    return api.residual_norms(h->data_ptr(), d->data_ptr(), delta_code, ptr(more[1]), ptr(more[2]), gate_rows, scale, ptr(more[0]), ho->data_ptr(),
                               quantized ? t.q.data_ptr() : ptr(out), quantized ? t.ld : n, quantized ? t.scales.data_ptr() : nullptr, rows,
                               static_cast<int>(n), eps, code, stream);
   });
@@ -643,7 +643,7 @@ PyObject* bind(PyObject*, PyObject* args) {
   find(api.int8_workspace_bytes, "lcq_int8_matmul_workspace_bytes");
   find(api.quantize_tokens, "lcq_quantize_tokens");
   find(api.silu_mul_tokens, "lcq_silu_mul_tokens");
-  find(api.residual_norms, "lcq_residual_norms");
+  find(api.residual_norms, "lcq_residual_norms_delta");
   if (!all) return PyErr_Format(PyExc_ImportError, "%s lacks an entry point", path);
   Py_INCREF(raise_fn);
   Py_INCREF(workspace_fn);

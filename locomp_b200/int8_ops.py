@@ -165,7 +165,8 @@ def residual_norms(hidden, delta, weight=None, eps: float = 1e-5, *, post_weight
 
     residual_rms_norm is the case without post_weight, gate and scale.  hidden, delta: [n] or [rows, n].  gate: [n], one value a channel,
     or [g, n] with rows % g == 0, each row for rows / g consecutive rows of hidden (a sequence's tokens; g = rows: its own for each).
-    Arithmetic is float32; hidden is rounded to its type as it is stored, and the second norm reads it so.
+    Arithmetic is float32; hidden is rounded to its type as it is stored, and the second norm reads it so.  All operands share hidden's type; delta
+    may be float32 beside it, as a product leaves it with out_dtype="f32", and is then rounded only as it is added.
     quantized=True: out is QuantizedTokens (see quantize_tokens).  weight=None: no norm follows, and the result is the new hidden."""
     if stream is None and not bf16 and isinstance(hidden, torch.Tensor):
         o = (out.q, out.scales) if isinstance(out, QuantizedTokens) else out
@@ -199,7 +200,10 @@ def residual_norms(hidden, delta, weight=None, eps: float = 1e-5, *, post_weight
             raise TypeError("hidden_out must be a device tensor")
         if hno.size != ho.size:
             raise ValueError(f"hidden_out must hold {ho.size} values, got {hno.size}")
-    kind, dev = _same(ho, do, hno, *parts.values())
+    kind, dev = _same(ho, hno, *parts.values())
+    if do.kind not in (kind, "f32"):
+        raise TypeError(f"delta must be {kind} as hidden is, or f32, got {do.kind}")
+    _same_device(ho, do)
     code = _float_kind(ho, "hidden")
     _require_cuda()
     with _on(dev, stream):
@@ -214,9 +218,9 @@ def residual_norms(hidden, delta, weight=None, eps: float = 1e-5, *, post_weight
             _same(ho, oo)
             out_ptr = oo.ptr
         ptr = {name: op.ptr for name, op in parts.items()}
-        _lib.check(_lib.lib().lcq_residual_norms(ho.ptr, do.ptr, ptr.get("post_weight"), ptr.get("gate"), gate_rows, float(scale),
-                                                 ptr.get("weight"), hno.ptr, out_ptr, ldo, scales, rows, n, float(eps), code,
-                                                 current_stream_ptr()))
+        _lib.check(_lib.lib().lcq_residual_norms_delta(ho.ptr, do.ptr, KIND_TO_CODE[do.kind], ptr.get("post_weight"), ptr.get("gate"), gate_rows,
+                                                       float(scale), ptr.get("weight"), hno.ptr, out_ptr, ldo, scales, rows, n, float(eps), code,
+                                                       current_stream_ptr()))
         return res if oo is None else _finish(oo, res)
 
 

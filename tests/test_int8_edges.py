@@ -289,3 +289,79 @@ def test_a_layer_of_weights_whose_rows_lie_on_one_another():
         k = w.shape[1]
         assert torch.equal(L.Int8Linear(w, scales)(x[:, :k].contiguous()), L.Int8Linear(w.contiguous(), scales)(x[:, :k].contiguous()))
     status_ok()
+
+
+# ------------------------------------------------------------------------------------------ float32 between operators
+MIXED = [(1, 1), (1, 576), (5, 100), (9, 512), (2, 513), (7, 1537), (4, 4096), (33, 264), (1, 8192), (3, 8200), (2, 16384), (3, 16392), (2, 20001), (1, 50000),
+         (600, 64), (1200, 1537), (400, 2048)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS[1:])
+@pytest.mark.parametrize("rows,n", MIXED)
+def test_residual_of_a_float32_delta(rows, n, kind):
+    """hidden of 16 bits, delta as a product leaves it in float32: rounded once, as the sum is stored.  Bounds as in test_rows_against_64_bits."""
+    g = gen(rows, n)
+
+    def draw(r, scale=1.0, plus=0.0, as_kind=kind):
+        return (torch.randn(r, n, device="cuda", generator=g) * scale + plus).to(as_kind)
+    x, delta, w, post = draw(rows), draw(rows, 3.0, 0.0, torch.float32), draw(1, 0.1, 1.0)[0], draw(1, 0.1, 1.0)[0]
+    for has_post, gate_rows, scale in ((True, 1, 0.5), (False, rows, -1.5), (True, 0, 1.0), (False, 0, 1.0)):
+        gate = draw(gate_rows, 0.5) if gate_rows else None
+        kw = dict(gate=gate, post_weight=post if has_post else None, scale=scale)
+        y = rms(delta.double(), post) if has_post else delta.double()
+        if gate_rows:
+            y = y * gate.double()
+        y = scale * y
+        ref = x.double() + y
+        hidden = torch.empty_like(x)
+        out = L.residual_norms(x, delta, w, hidden_out=hidden, **kw)
+        assert out.dtype == kind
+        slack = REL * y.abs() + 2.0 ** -24 * ref.abs()
+        assert bool(((hidden.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * slack + 2.0 ** -25).all())
+        normed = rms(hidden.double(), w)
+        assert bool(((out.double() - normed).abs() <= (HALF_STEP[kind] + 1.01 * REL) * normed.abs() + 2.0 ** -25).all())
+        again = x.clone()
+        tokens = L.residual_norms(again, delta, w, quantized=True, **kw)
+        assert torch.equal(again, hidden)
+        check_tokens(tokens, normed)
+        once = x.clone()
+        assert L.residual_norms(once, delta, **kw) is once and torch.equal(once, hidden)
+        if has_post and gate_rows:                            # the general path, and rows off 16 bytes
+            once = x.clone()
+            assert torch.equal(L.residual_norms(L.DeviceTensor(once), delta, w, **kw), out) and torch.equal(once, hidden)
+            off = torch.empty(rows * n + 1, device="cuda")[1:].view(rows, n).copy_(delta)
+            once = x.clone()
+            moved = L.residual_norms(once, off, w, **kw)
+            assert bool(((once.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * slack + 2.0 ** -25).all())
+            normed = rms(once.double(), w)
+            assert bool(((moved.double() - normed).abs() <= (HALF_STEP[kind] + 1.01 * REL) * normed.abs() + 2.0 ** -25).all())
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_residual_refuses_other_types_of_delta():
+    f = {k: torch.randn(4, 64, device="cuda").to(k) for k in KINDS}
+    for hidden in KINDS:
+        for delta in KINDS:
+            if delta in (hidden, torch.float32):
+                assert L.residual_norms(f[hidden].clone(), f[delta], f[hidden][0]).dtype == hidden
+            else:
+                with pytest.raises(TypeError, match="delta must be"):
+                    L.residual_norms(f[hidden].clone(), f[delta], f[hidden][0])
+            if delta != hidden:                               # nothing else may differ
+                for kw in (dict(weight=f[delta][0]), dict(post_weight=f[delta][0]), dict(gate=f[delta][0]), dict(hidden_out=f[delta].clone()),
+                           dict(weight=f[hidden][0], out=f[delta].clone())):
+                    with pytest.raises(TypeError, match="one dtype"):
+                        L.residual_norms(f[hidden].clone(), f[hidden], **kw)
+    with pytest.raises(TypeError, match="delta must be"):
+        L.residual_norms(f[torch.float16].clone(), torch.zeros(4, 64, dtype=torch.int8, device="cuda"))
+
+
+def test_residual_entry_checks_the_type_of_delta():
+    lib, p = _lib.lib(), ctypes.c_void_p(4096)
+    for dtype in range(3):
+        for delta in range(-1, 5):
+            rc = lib.lcq_residual_norms_delta(p, p, delta, None, None, 0, 1.0, p, p, p, 8, None, 0, 8, 1e-5, dtype, None)
+            assert rc == (0 if delta in (dtype, 0) else _lib.ERR_BAD_ARG)
+    assert lib.lcq_residual_norms_delta(p, p, 0, None, p, 4, 1.0, p, p, p, 8, None, 6, 8, 1e-5, 1, None) == _lib.ERR_BAD_ARG
