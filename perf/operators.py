@@ -209,7 +209,7 @@ def _own(s):
     t = L.quantize_tokens(s["input"], s["in_weight"], EPS)
     gate_up = L.int8_matmul(t.q, t.scales, s["w1"], s["s1"], out_dtype="f32")      # to be quantised next: 16 bits would move q by a step here and there
     t = L.silu_mul_tokens(gate_up[:, :s["inter"]], gate_up[:, s["inter"]:])
-    down = L.int8_matmul(t.q, t.scales, s["w2"], s["s2"], out_dtype=s["x"])
+    down = L.int8_matmul(t.q, t.scales, s["w2"], s["s2"], out_dtype="f32")         # to be normalised and added: rounded once, as the stream is stored
     normed = L.residual_norms(s["input"], down, s["weight"], EPS, post_weight=s["post_weight"], scale=0.5, hidden_out=s["hidden_out"])
     return s["hidden_out"], normed
 
