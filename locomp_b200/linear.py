@@ -208,8 +208,6 @@ class DecodeStack:
         def norm():
             return (1 + 0.1 * torch.randn(hidden, device=device, generator=g)).to(dtype)
 
-        def empty(n):
-            return torch.empty(1, n, dtype=dtype, device=device)
         self.table = (torch.randn(vocab, hidden, device=device, generator=g) * 0.02).to(dtype)
         self.token, self.next_token = (torch.zeros(1, dtype=torch.int32, device=device) for _ in range(2))
         self.hidden = torch.zeros(1, hidden, dtype=dtype, device=device)
@@ -218,8 +216,8 @@ class DecodeStack:
         first = norm()
         self.norms = [first]
 
-        def product(lin, tokens):
-            out = empty(lin.out_features)
+        def product(lin, tokens, kind=torch.float32):  # (float32 up to the next quantisation or the residual: 16 bits would move tokens by a step)
+            out = torch.empty(1, lin.out_features, dtype=kind, device=device)
             self.calls.append((lin, tokens, out))
             self.ops.append(lambda: lin(tokens, out=out))
             return out
@@ -237,7 +235,7 @@ class DecodeStack:
             gu = product(layer(2 * inter, hidden), self.normed)
             self.ops.append(lambda gu=gu: silu_mul_tokens(gu[:, :inter], gu[:, inter:], out=self.mlp))
             to_next_block(product(layer(hidden, inter), self.mlp))
-        self.logits = product(layer(vocab, hidden), self.normed)
+        self.logits = product(layer(vocab, hidden), self.normed, dtype)
         self.ops.append(lambda: D.argmax(self.logits, out=self.next_token))
 
     def _one_kernel(self, x_q, layers, hidden, inter, qd, qkv, vocab):

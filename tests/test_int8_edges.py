@@ -365,3 +365,39 @@ def test_residual_entry_checks_the_type_of_delta():
             rc = lib.lcq_residual_norms_delta(p, p, delta, None, None, 0, 1.0, p, p, p, 8, None, 0, 8, 1e-5, dtype, None)
             assert rc == (0 if delta in (dtype, 0) else _lib.ERR_BAD_ARG)
     assert lib.lcq_residual_norms_delta(p, p, 0, None, p, 4, 1.0, p, p, p, 8, None, 6, 8, 1e-5, 1, None) == _lib.ERR_BAD_ARG
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS[1:])
+def test_decode_stack_rounds_where_something_is_stored(kind):
+    """From tokens to tokens and to the stream against 64 bits, across the product and what follows it: nothing is rounded to 16 bits between."""
+    inter = 1536
+    st = L.DecodeStack(layers=1, hidden=576, inter=inter, vocab=1000, fused=True, glue=True, int8=True, dtype=kind, post_norms=True, residual_scale=0.5, seed=2)
+    assert [out.dtype for _, _, out in st.calls] == [torch.float32] * 4 + [kind]
+    st.token.fill_(7)
+    ops, norms, calls = iter(st.ops), iter(st.norms), iter(st.calls)
+
+    def product():
+        lin, tokens, _ = next(calls)
+        next(ops)()
+        return tokens.q.double() @ lin.w.double().t() * tokens.scales.double()[:, None] * lin.scales.double()
+
+    def block_end(delta):
+        before = st.hidden.double()
+        next(ops)()
+        y = 0.5 * rms(delta, next(norms))
+        ref = before + y
+        # a product in float32 is off by 3 * 2^-24, its norm by REL and less than that again
+        assert bool(((st.hidden.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * (2 * REL * y.abs() + 2.0 ** -24 * ref.abs()) + 2.0 ** -25).all())
+        check_tokens(st.normed, rms(st.hidden.double(), next(norms)))
+    next(ops)()
+    next(ops)()
+    next(norms)
+    product()
+    block_end(product())
+    gu = product()
+    next(ops)()
+    a, b = gu[:, :inter], gu[:, inter:]
+    check_tokens(st.mlp, a * torch.sigmoid(a) * b)
+    block_end(product())
+    status_ok()
