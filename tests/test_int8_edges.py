@@ -401,3 +401,23 @@ def test_decode_stack_rounds_where_something_is_stored(kind):
     check_tokens(st.mlp, a * torch.sigmoid(a) * b)
     block_end(product())
     status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS[1:])
+def test_half_way_quotients_of_normed_tokens(kind):
+    """Of 16-bit rows x weight is exact, and quotients v / (amax / 127) that are half-integers are common.  No float32 scale makes all of them ties to even
+    (a float32 division has 15 % of those of amax / 2 wrong, over all 8-bit amax), but a reciprocal without the quotient's rounding had half."""
+    g = gen(11)
+    x = torch.randn(20000, 512, device="cuda", generator=g).to(torch.bfloat16).to(kind)          # 8 bits of mantissa in either type
+    w = torch.tensor([0.5, 1.0, 2.0], device="cuda", dtype=kind)[torch.randint(0, 3, (512,), device="cuda", generator=g)]
+    v = x.double() * w.double()
+    amax = v.abs().amax(-1, keepdim=True)
+    half = (254 * v / amax).round()
+    ties = (half * amax == 254 * v) & (half.remainder(2) == 1)
+    even = (127 * v[ties] / amax.expand_as(v)[ties]).round()
+    assert int(ties.sum()) > 500
+    for t in (L.quantize_tokens(x, w), L.residual_norms(torch.zeros_like(x), x, w, quantized=True)):
+        check_tokens(t, rms(x.double(), w))
+        assert int((t.q[ties].double() != even).sum()) <= 0.25 * int(ties.sum())
+    status_ok()
