@@ -149,7 +149,10 @@ template <bool PAIRS> __device__ __forceinline__ void add_scaled8(float (&v)[8],
     v[j + 1] = r.y;
   }
 }
-struct Squares {             // two sums, the same ones either way
+// Two sums, the same ones either way.  A row in chunks adds each chunk's to a double, so that the error does not grow with the row: at most 32 squares meet in
+// float32 before the tree of shuffles, whatever its length (2^24 values of 0.7 in one float32 sum a thread: the norm 1.1e-4 off).
+struct Squares {
+  double chunks = 0.0;
   uint64_t two = 0;
   float one = 0.0f, other = 0.0f;
   template <bool PAIRS> __device__ __forceinline__ void add(const float (&v)[8]) {
@@ -168,6 +171,12 @@ struct Squares {             // two sums, the same ones either way
     const float2 r = unpack_pair(two);
     return PAIRS ? r.x + r.y : one + other;
   }
+  template <bool PAIRS> __device__ __forceinline__ void end_chunk() {
+    chunks += static_cast<double>(sum<PAIRS>());
+    two = 0;
+    one = other = 0.0f;
+  }
+  template <bool PAIRS, bool WHOLE> __device__ __forceinline__ float total() const { return WHOLE ? sum<PAIRS>() : static_cast<float>(chunks); }
 };
 
 // The larger magnitude, or NaN where there is one.
@@ -312,8 +321,9 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
         y[e].get(v);
         squares.template add<PAIRS>(v);
       }
+      if (!WHOLE) squares.template end_chunk<PAIRS>();
     }
-    float ss = squares.template sum<PAIRS>();
+    float ss = squares.template total<PAIRS, WHOLE>();
     reduce_row<WARP_ROW>(ss, red[0]);
     rd = rsqrtf(ss / static_cast<float>(n) + p.eps);
   }
@@ -373,9 +383,10 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
         magnitudes(v);
       }
     }
+    if (!WHOLE && NORMED) squares.template end_chunk<PAIRS>();
   }
   if (!QUANT && !weight) return;                     // RESIDUAL without a norm after it
-  float ss = squares.template sum<PAIRS>();
+  float ss = squares.template total<PAIRS, WHOLE>();
   reduce_row<WARP_ROW>(ss, amax, red[1]);
   const float rr = NORMED ? rsqrtf(ss / static_cast<float>(n) + p.eps) : 1.0f;
   const bool finite = amax < __uint_as_float(0x7F800000u);       // (false for NaN)

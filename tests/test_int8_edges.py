@@ -421,3 +421,22 @@ def test_half_way_quotients_of_normed_tokens(kind):
         check_tokens(t, rms(x.double(), w))
         assert int((t.q[ties].double() != even).sum()) <= 0.25 * int(ties.sum())
     status_ok()
+
+
+# ------------------------------------------------------------------------------------------ long rows
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_millions(kind):
+    """One bound for rows of any length: equal values, whose rounding errors all have one sign in a running sum."""
+    for n, value in ((1 << 22, 1.1), (1 << 24, 0.7), ((1 << 24) + 3, 1.7)):
+        x = torch.full((1, n), value, device="cuda").to(kind)
+        ramp = (1 + (torch.arange(n, device="cuda") % 5) * 0.25).to(kind)
+        want = rms(x.double(), ramp)
+        check_tokens(L.quantize_tokens(x, ramp), want)
+        hidden = torch.zeros_like(x)
+        out = L.residual_norms(hidden, x, ramp, post_weight=torch.ones_like(ramp))
+        assert bool(((hidden.double() - rms(x.double(), torch.ones_like(ramp))).abs() <= HALF_STEP[kind] + (1 + HALF_STEP[kind]) * REL).all())
+        normed = rms(hidden.double(), ramp)
+        assert bool(((out.double() - normed).abs() <= (HALF_STEP[kind] + 1.01 * REL) * normed).all())
+        del want, normed
+    status_ok()
