@@ -448,6 +448,8 @@ int launch_form(const Args& p, int threads, cudaStream_t st) {
 //                                     the copy rate)
 //   E = 8                             16-bit rows up to 32,768 of one operand (4000 x 28,672 quantised: 69; E = 4 93); of two, E = 4 in twice the threads
 //                                     (1000 x 28,672 SILU_MUL: 39; E = 8 44, in chunks 58)
+//   in chunks, E = 2                  longer rows, two blocks an SM (1000 x 50,001 bfloat16 SILU_MUL 150, one block 156; 1000 x 50,000 RESIDUAL 100 and 141); one for two
+//                                     operands in float32, which do not fit into 64 registers (1000 x 50,000 RESIDUAL 206, two blocks 303; 64 x 20,001 14 and 30)
 template <typename T, typename D, int OP, bool QUANT, bool ALIGNED>
 int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
   constexpr bool HALF = sizeof(D) == 2, ONE = OP == ROWS || OP == NORM_ROWS;
@@ -473,7 +475,7 @@ int launch_aligned(const Args& p, int sm_count, cudaStream_t st) {
       if (span <= 32768) return launch_form<T, D, OP, QUANT, ALIGNED, 4, false, true, 1024, 1>(p, threads(4), st);
     }
   }
-  return launch_form<T, D, OP, QUANT, ALIGNED, 2, false, false, 512, 2>(p, 512, st);
+  return launch_form<T, D, OP, QUANT, ALIGNED, 2, false, false, 512, HALF || ONE ? 2 : 1>(p, 512, st);
 }
 
 // Octets as they lie where every row of every operand starts on 16 bytes (of q: on 8) and holds whole ones.
