@@ -440,3 +440,57 @@ def test_rows_of_millions(kind):
         assert bool(((out.double() - normed).abs() <= (HALF_STEP[kind] + 1.01 * REL) * normed).all())
         del want, normed
     status_ok()
+
+
+# longer than a block's registers hold in any type
+LONG = [(2, 32769), (1, 40001), (3, 50003), (2, 65537 + 6)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("rows,n", LONG)
+@pytest.mark.parametrize("place", [0, 1, 5])
+def test_long_rows_off_16_bytes(rows, n, kind, place):
+    """Rows that are read again for each pass over them, written from the first value on 16 bytes on, at other places in every operand.  Bounds as in
+    test_rows_against_64_bits."""
+    g = gen(rows, n, place)
+
+    def draw(r, scale=1.0, plus=0.0, at=0):
+        flat = torch.empty(r * n + 8, device="cuda", dtype=kind)
+        return flat[at:at + r * n].view(r, n).copy_(torch.randn(r, n, device="cuda", generator=g) * scale + plus)
+    x, delta = draw(rows, at=place), draw(rows, 3.0, at=(place + 3) % 8)
+    w, post, gate = draw(1, 0.1, 1.0, at=(place + 1) % 8)[0], draw(1, 0.1, 1.0, at=place)[0], draw(rows, 0.5, at=(place + 2) % 8)
+    t = L.quantize_tokens(x)
+    whole = L.quantize(x.clone(), n, bits=8)
+    assert torch.equal(t.q, whole.w) and torch.equal(t.scales, whole.scales.view(-1))
+    check_tokens(L.quantize_tokens(x, w), rms(x.double(), w))
+    a, b = x.double(), delta.double()
+    check_tokens(L.silu_mul_tokens(x, delta), a * torch.sigmoid(a) * b)
+    q = torch.full((rows, n + 32), 77, dtype=torch.int8, device="cuda")
+    out = L.QuantizedTokens(q[:, 3:3 + n], torch.empty(rows, device="cuda"))
+    L.silu_mul_tokens(x, delta, out=out)
+    check_tokens(out, a * torch.sigmoid(a) * b)
+    assert bool((q[:, :3] == 77).all()) and bool((q[:, 3 + n:] == 77).all())
+    for has_post, gated, scale in ((True, True, 0.5), (False, True, -1.5), (True, False, 1.0), (False, False, 1.0)):
+        kw = dict(post_weight=post if has_post else None, gate=gate if gated else None, scale=scale)
+        y = rms(b, post) if has_post else b
+        y = scale * (y * gate.double() if gated else y)
+        ref = a + y
+        buf = torch.full((rows * n + 16,), 9.0, device="cuda", dtype=kind)
+        hidden = buf[7:7 + rows * n].view(rows, n)
+        norm = torch.full((rows * n + 16,), 9.0, device="cuda", dtype=kind)
+        written = norm[2:2 + rows * n].view(rows, n)
+        assert L.residual_norms(x, delta, w, hidden_out=hidden, out=written, **kw) is written
+        slack = REL * y.abs() + 2.0 ** -24 * ref.abs()
+        assert bool(((hidden.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * slack + 2.0 ** -25).all())
+        normed = rms(hidden.double(), w)
+        assert bool(((written.double() - normed).abs() <= (HALF_STEP[kind] + 1.01 * REL) * normed.abs() + 2.0 ** -25).all())
+        for edge in (buf[:7], buf[7 + rows * n:], norm[:2], norm[2 + rows * n:]):
+            assert bool((edge == 9).all())
+        again = x.clone()
+        check_tokens(L.residual_norms(again, delta, w, quantized=True, **kw), rms(again.double(), w))
+        # (not the bits of `hidden`: octets are counted from where the written row lies on 16 bytes, so the squares of delta meet in another order and each
+        # result has the bound above by itself)
+        assert bool(((again.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * slack + 2.0 ** -25).all())
+        assert has_post or torch.equal(again, hidden)                    # no sum comes before hidden without the norm of delta
+    status_ok()
