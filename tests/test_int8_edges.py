@@ -494,3 +494,45 @@ def test_long_rows_off_16_bytes(rows, n, kind, place):
         assert bool(((again.double() - ref).abs() <= HALF_STEP[kind] * ref.abs() + (1 + HALF_STEP[kind]) * slack + 2.0 ** -25).all())
         assert has_post or torch.equal(again, hidden)                    # no sum comes before hidden without the norm of delta
     status_ok()
+
+
+# ------------------------------------------------------------------------------------------ one after the other
+@pytest.mark.gpu
+@pytest.mark.parametrize("m,n,k", [(1, 8192, 2048), (1, 40000, 576), (4, 8192, 2048), (4, 8192, 2041), (16, 8192, 2048), (300, 8192, 2048), (300, 3000, 2041), (16, 9000, 2041)])
+def test_product_of_operands_that_a_kernel_ahead_is_still_writing(m, n, k):
+    """Weights, tokens and both scales come from kernels that let their successor start before they have written anything: each of the product's kernels (dp4a, warp MMAs,
+    the ring, and the copy of rows off 16 bytes) has to wait for them.  Other values each time."""
+    g = gen(m, n, k)
+    weights = [torch.randn(n, k, device="cuda", generator=g) for _ in range(3)]
+    tokens = [torch.randn(m, k, device="cuda", generator=g) for _ in range(2)]
+    want = []
+    for i in range(6):
+        x, w = L.quantize_tokens(tokens[i % 2]), L.quantize_tokens(weights[i % 3])
+        want.append(x.q.double() @ w.q.double().t() * x.scales.double()[:, None] * w.scales.double())
+    w = L.QuantizedTokens(torch.zeros(n, k, dtype=torch.int8, device="cuda"), torch.zeros(n, device="cuda"))
+    x = L.quantize_tokens(tokens[0])
+    outs = torch.empty(24, m, n, device="cuda")
+
+    def chain():
+        for i in range(24):
+            if i % 4 < 2:                                     # now the weights last, now the tokens
+                L.quantize_tokens(tokens[i % 2], out=x)
+                L.quantize_tokens(weights[i % 3], out=w)
+            else:
+                L.quantize_tokens(weights[i % 3], out=w)
+                L.quantize_tokens(tokens[i % 2], out=x)
+            L.int8_matmul(x.q, x.scales, w.q, w.scales, out=outs[i])
+    torch.cuda.synchronize()
+    chain()
+    for i in range(24):
+        check_product(outs[i], want[i % 6], torch.float32)
+    direct = outs.clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        chain()
+    for _ in range(2):
+        outs.zero_()
+        graph.replay()
+        assert torch.equal(outs, direct)
+    status_ok()
