@@ -6,6 +6,7 @@ import ctypes
 import itertools
 import os
 import random
+import threading
 
 import pytest
 import torch
@@ -535,4 +536,39 @@ def test_product_of_operands_that_a_kernel_ahead_is_still_writing(m, n, k):
         outs.zero_()
         graph.replay()
         assert torch.equal(outs, direct)
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_a_threads_first_call():
+    """A thread that has made no CUDA call yet has no context, which the driver wants for a tensor map."""
+    g = gen(12)
+    w4 = torch.randint(0, 256, (2048, 512), dtype=torch.uint8, device="cuda", generator=g)
+    s4 = (torch.rand(2048, 32, device="cuda", generator=g) * 0.02).half()
+    calls = []
+    for m in (1, 16, 300):
+        a = torch.randn(m, 1024, device="cuda", generator=g).half()
+        calls.append((lambda out, a=a: L.quantized_matmul(a, w4, s4, 32, out=out), L.quantized_matmul(a, w4, s4, 32)))
+    for size in ((1, 512, 1024), (8, 512, 1024), (16, 512, 1024), (300, 512, 1024), (16, 512, 1001), (300, 512, 1001)):
+        x, xs, w, ws, _ = product_case(*size)
+        calls.append((lambda out, c=(x, xs, w, ws): L.int8_matmul(*c, out=out), L.int8_matmul(x, xs, w, ws)))
+    x = torch.randn(4, 512, device="cuda", generator=g).half()
+    norm = torch.ones(512, device="cuda").half()
+    calls.append((lambda out: L.residual_norms(x, x, norm, hidden_out=torch.empty_like(x), out=out), L.residual_norms(x, x, norm, hidden_out=torch.empty_like(x))))
+    torch.cuda.synchronize()
+    for call, want in calls:
+        out, failed = torch.zeros_like(want), []
+        torch.cuda.synchronize()
+
+        def work():
+            try:
+                call(out)
+            except Exception as e:
+                failed.append(e)
+        t = threading.Thread(target=work)
+        t.start()
+        t.join()
+        assert not failed, failed
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
     status_ok()
