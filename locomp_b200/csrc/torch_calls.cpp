@@ -21,7 +21,6 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/cuda/EmptyTensor.h>
-#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -511,25 +510,18 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const size_t bytes = given->nbytes();
     rc = unlocked([&] { return call(ptr, bytes); });
     if (rc == LCQ_ERR_WORKSPACE) return not_implemented();
-  } else if (c10::cuda::currentStreamCaptureStatusMayInitCtx() != c10::cuda::CaptureStatus::None) {
-    rc = unlocked([&] { return call(nullptr, 0); });
-    if (rc == LCQ_ERR_WORKSPACE) return not_implemented();   // (the general path gives the graph scratch of its own)
   } else {
-    Scratch& scratch = scratches[{dev, reinterpret_cast<uintptr_t>(stream)}];
-    NoGil released;
-    const std::lock_guard<std::recursive_mutex> held(scratch.lock);
-    rc = call(scratch.ptr, scratch.bytes);
-    if (rc == LCQ_ERR_WORKSPACE) {
-      released.end();
-      const auto on_16 = [](const void* rows, int64_t n, int64_t ld) { return reinterpret_cast<uintptr_t>(rows) % 16 == 0 && (n == 1 || ld % 16 == 0); };
-      const size_t need = api.int8_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), on_16(xp, M, ldx), on_16(wp, N, ldw));
-      PyObject* r = PyObject_CallFunction(make_workspace, "niK", static_cast<Py_ssize_t>(need), dev,
-                                          static_cast<unsigned long long>(reinterpret_cast<uintptr_t>(stream)));
-      if (!r) return nullptr;
-      Py_DECREF(r);
-      released.again();
-      rc = call(scratch.ptr, scratch.bytes);
-    }
+    // Memory of this call's own, given back in the stream's order (under capture: the graph's): growing the stream's scratch would free what a graph of int4
+    // products holds the address of.
+    const auto on_16 = [](const void* rows, int64_t n, int64_t ld) { return reinterpret_cast<uintptr_t>(rows) % 16 == 0 && (n == 1 || ld % 16 == 0); };
+    const bool x_on_16 = on_16(xp, M, ldx), w_on_16 = on_16(wp, N, ldw);
+    size_t need = 0;
+    if (!x_on_16 || !w_on_16) need = api.int8_workspace_bytes(static_cast<int>(M), static_cast<int>(N), static_cast<int>(K), x_on_16, w_on_16);
+    if (need == static_cast<size_t>(-1)) need = 0;           // (the call says why)
+    at::Tensor scratch;
+    if (need) scratch = empty({static_cast<int64_t>(need)}, at::kByte, *x);
+    void* ptr = need ? scratch.data_ptr() : nullptr;
+    rc = unlocked([&] { return call(ptr, need); });
   }
   return args[4] == Py_None ? finish(rc, std::move(made)) : finish(rc, args[4]);
 }

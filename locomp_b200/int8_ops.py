@@ -22,8 +22,7 @@ import torch
 from . import _lib
 from .decode_ops import _finish, _same
 from .ops import _float_kind, _same_device
-from .tensor import (KIND_TO_CODE, KIND_TO_TORCH, Operand, _require_cuda, current_stream_ptr, locked_workspace, resolve,
-                     workspace)
+from .tensor import KIND_TO_CODE, KIND_TO_TORCH, Operand, _require_cuda, current_stream_ptr, resolve
 
 
 @dataclass
@@ -233,8 +232,8 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
     quantize_tokens gives them for a batch of sequences: [..., K] with x_scales of the shape [...].  Rows of x and w may be
     further apart than K; those that do not start on 16 bytes (K % 16 != 0 in contiguous storage) cost a copy.
     Returns a torch CUDA tensor [N], [M, N] or [..., N] of out_dtype ("f32", "f16", "bf16"; default "f16") or `out`.  K is at most 131071.
-    Scratch is needed for such copies only: workspace_buf, or this package's buffer of the stream; under CUDA-graph capture the graph's own memory,
-    so that no two graphs share it."""
+    Scratch is needed for such copies only: workspace_buf, or memory that the call takes from torch's allocator on its stream; under CUDA-graph capture
+    that is the graph's own, so that no two graphs share it."""
     if isinstance(x, torch.Tensor) and stream is None:
         res = _lib.calls.int8_matmul(x, x_scales, w, w_scales, out, -1 if out_dtype is None else KIND_TO_CODE.get(out_dtype, -2), workspace_buf)
         if res is not NotImplemented:
@@ -287,11 +286,8 @@ def int8_matmul(x, x_scales, w, w_scales, *, out=None, out_dtype: Optional[str] 
             if workspace_buf.numel() * workspace_buf.element_size() < need or workspace_buf.device.index != dev or not workspace_buf.is_contiguous():
                 raise ValueError(f"workspace_buf must hold {need} bytes on cuda:{dev}")
             launch(workspace_buf)
-        elif torch.cuda.is_current_stream_capturing():
-            launch(torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev)))
         else:
-            with locked_workspace(dev, sp):
-                launch(workspace(need, dev, sp))
+            launch(torch.empty(need, dtype=torch.uint8, device=torch.device("cuda", dev)))
         if oo.host is not None:
             return _finish(oo, res)
     return res

@@ -6,6 +6,7 @@ import ctypes
 import itertools
 import os
 import random
+import sys
 import threading
 
 import pytest
@@ -14,6 +15,8 @@ import torch
 import locomp_b200 as L
 from locomp_b200 import _lib
 from test_int8_path import HALF_STEP, KINDS, NAMES, REL, check_product, check_tokens, gen, plan, product_case, rms, status_ok
+
+tensor_module = sys.modules["locomp_b200.tensor"]        # (the package's `tensor` is a function)
 
 
 # ------------------------------------------------------------------------------------------ views
@@ -571,4 +574,69 @@ def test_a_threads_first_call():
         assert not failed, failed
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_product_leaves_the_streams_scratch_to_the_graphs_that_hold_it():
+    """A graph of int4 products holds the address of its stream's scratch.  The int8 product's copies used to make that buffer grow, which gave the old one to whoever
+    allocated next."""
+    g, side = gen(13), torch.cuda.Stream()
+    w4 = torch.randint(0, 256, (20000, 2048), dtype=torch.uint8, device="cuda", generator=g)
+    s4 = (torch.rand(20000, 128, device="cuda", generator=g) * 0.02).half()
+    a = torch.randn(16, 4096, device="cuda", generator=g).half()
+    want, out = L.quantized_matmul(a, w4, s4, 32), torch.empty(16, 20000, dtype=torch.float16, device="cuda")
+    x, xs, w, ws, ref = product_case(16, 9000, 4101)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        L.quantized_matmul(a, w4, s4, 32, out=out)
+        side.synchronize()
+        with torch.cuda.graph(graph, stream=side):
+            L.quantized_matmul(a, w4, s4, 32, out=out)
+        before = {k: t.data_ptr() for k, t in tensor_module._workspaces.items()}
+        for form in (x, L.DeviceTensor(x)):
+            check_product(L.int8_matmul(form, xs, w, ws, out_dtype="f32"), ref, torch.float32)
+            check_product(L.int8_matmul(form, xs, w, ws, out_dtype="f32", stream=side), ref, torch.float32)
+        canaries = [torch.full((1 << 18,), 5, dtype=torch.int32, device="cuda") for _ in range(8)]
+        out.zero_()
+        for _ in range(3):
+            graph.replay()
+        side.synchronize()
+    assert {k: t.data_ptr() for k, t in tensor_module._workspaces.items()} == before
+    assert torch.equal(out, want) and all(bool((c == 5).all()) for c in canaries)
+    status_ok()
+
+
+@pytest.mark.gpu
+def test_products_that_copy_share_a_stream_and_two_graphs():
+    """Copies of two threads on one stream, and of two graphs that are replayed side by side: each has memory of its own."""
+    cases = [product_case(m, n, k) for m, n, k in ((16, 9000, 2049), (40, 5000, 1001), (300, 3000, 577))]
+    graphs, outs, streams = [], [], [torch.cuda.Stream() for _ in cases]
+    for x, xs, w, ws, _ in cases:
+        outs.append(L.int8_matmul(x, xs, w, ws, out_dtype="f32"))
+        graphs.append(torch.cuda.CUDAGraph())
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[-1]):
+            for _ in range(4):
+                L.int8_matmul(x, xs, w, ws, out=outs[-1])
+    for _ in range(10):
+        for graph, stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+    torch.cuda.synchronize()
+    for y, case in zip(outs, cases):
+        check_product(y, case[4], torch.float32)
+    wrong = []
+
+    def work(i):
+        ys = [L.int8_matmul(*cases[(i + j) % 3][:4], out_dtype="f32") for j in range(30)]
+        torch.cuda.current_stream().synchronize()
+        wrong.extend((i, j) for j, y in enumerate(ys) if not torch.equal(y, outs[(i + j) % 3]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
     status_ok()
