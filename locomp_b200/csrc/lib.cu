@@ -796,7 +796,13 @@ static int check_int8_tiling(const int8_gemm::Tiling& t, int M, int N, int K, in
     return wrong("cluster");
   if (t.split == 1 && t.cg * t.teams > sm_count) return wrong("more CTAs than SMs");
   const int unit = 16, units = (M + unit - 1) / unit;                     // of tokens
-  std::vector<int> stages(static_cast<size_t>(units) * t.tn, 0);          // stages of K that each unit of each channel tile has had
+  std::vector<int> stages;                                                // stages of K that each unit of each channel tile has had
+  try {
+    stages.resize(static_cast<size_t>(units) * t.tn, 0);
+  } catch (const std::bad_alloc&) {
+    set_error("int8 plan: no memory to replay %lld pieces of tiles", static_cast<long long>(units) * t.tn);
+    return LCQ_ERR_UNSUPPORTED;
+  }
   for (int team = 0; team < t.teams; ++team) {
     int items = 0;
     for (Walk w(p, team); w.next(p); ++items) {

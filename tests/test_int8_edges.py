@@ -6,6 +6,7 @@ import ctypes
 import itertools
 import os
 import random
+import subprocess
 import sys
 import threading
 
@@ -177,6 +178,16 @@ def test_sizes_that_an_int_does_not_hold_are_refused():
         with pytest.raises(ctypes.ArgumentError, match="does not fit"):
             call()
     assert lib.lcq_residual_norms(None, None, None, None, 0, 1.0, None, None, None, 0, None, big, 0, 1e-5, 0, None) == 0      # rows are 64 bits
+
+
+def test_a_plan_without_the_memory_to_check_it_is_refused():
+    """An exception may not leave a C entry: 62500 x 7813 pieces, in a process of little memory."""
+    code = ("import ctypes, resource, sys\n"
+            "lib = ctypes.CDLL(sys.argv[1])\n"
+            "here = int(open('/proc/self/statm').read().split()[0]) * resource.getpagesize()\n"
+            "resource.setrlimit(resource.RLIMIT_AS, (here + (1 << 29), resource.getrlimit(resource.RLIMIT_AS)[1]))\n"
+            "sys.exit(10 + lib.lcq_int8_matmul_plan_check(1000000, 1000000, 64, 148, 1, None))\n")
+    assert subprocess.run([sys.executable, "-c", code, _lib.LIB_PATH], timeout=120).returncode == 10 + _lib.ERR_UNSUPPORTED
 
 
 @pytest.mark.gpu
