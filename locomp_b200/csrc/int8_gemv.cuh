@@ -13,7 +13,7 @@
 // Either way the tokens come out of L1, where all rows of an SM's warps find them, and there is no ring to fill, no tensor memory to allocate and no accumulator to
 // hand over.  As in int8_gemm.cuh, the first weights are fetched into L2 while the kernel ahead still runs, and read after it has completed.
 //
-// us, replayed graphs, this / int8_gemm.cuh: 1 x 2048 -> 2048 2.6 / 5.4, 1 x 14336 -> 4096 12.1 / 13.6, 1 x 8192 -> 28672 38.7 / 41, 1 x 2048 -> 49152 20.0 / 18.1;
+// us, replayed graphs, this / int8_gemm.cuh: 1 x 2048 -> 2048 2.6 / 5.4, 1 x 14336 -> 4096 12.1 / 13.6, 1 x 8192 -> 28672 38.7 / 41;
 // 8 x 2048 -> 2048 3.4 / 5.1, 8 x 4096 -> 4096 6.1 / 7.3, 8 x 14336 -> 4096 14.8 / 13.3; rows off 16 bytes (there with their copy): 8 x 4104 -> 28672 42 / 71.
 #pragma once
 #include "int8_gemm.cuh"
@@ -205,9 +205,13 @@ int launch_t(Params& p, bool on_16, int sm_count, cudaStream_t st) {
   return launch_kernel(on_16 ? int8_mma_kernel<OT, true> : int8_mma_kernel<OT, false>, blocks(), p, st);
 }
 // Whether these kernels take the call: one or two tokens, up to eight where little is read (further on the tensor cores' ring streams better, see above) or
-// where rows off 16 bytes would have to be copied.
+// where rows off 16 bytes would have to be copied.  Not one or two tokens of many rows of 1025 .. 4095 bytes: a warp's loads reach over 4096 bytes, and what they have on
+// their way of such a row is less.  us in graphs, this / ring: 1 x 1536 -> 28672 11.1 / 9.2, -> 151936 51 / 38; 1 x 2048 -> 16384 8.7 / 8.6, -> 49152 19.6 / 17.9;
+// 1 x 2560 -> 151936 69 / 60; but 1 x 2048 -> 8192 5.0 / 6.8, 1 x 1024 -> 65536 12.2 / 12.8, 1 x 4096 -> 49152 30.6 / 33.3, 1 x 8192 -> 28672 33 / 41.
 inline bool takes(int M, int N, int K, bool on_16) {
-  return M <= 2 || (M <= MAX_M && (!on_16 || (K <= 4096 && static_cast<long long>(N) * K <= (20ll << 20))));
+  const long long bytes = static_cast<long long>(N) * K;
+  if (M <= 2) return !on_16 || K <= 1024 || K >= 4096 || bytes < (32ll << 20);
+  return M <= MAX_M && (!on_16 || (K <= 4096 && bytes <= (20ll << 20)));
 }
 inline int launch(const int8_gemm::Operands& o, int M, int N, int K, int sm_count, cudaStream_t st) {
   Params p = {static_cast<const uint8_t*>(o.x), static_cast<const uint8_t*>(o.w), o.ldx, o.ldw, o.x_scales, o.w_scales, o.out, M, N, K, o.w_scale_dtype, 1};

@@ -651,3 +651,13 @@ def test_products_that_copy_share_a_stream_and_two_graphs():
         t.join()
     assert not wrong
     status_ok()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 2, 3])
+def test_few_tokens_on_either_side_of_each_kernels_range(m):
+    """One or two tokens go to dp4a, but for many rows of 1025 to 4095 bytes; three to warp MMAs up to 20 Mi weights.  Sizes next to each border."""
+    for k, n in ((1024, 32768), (1025, 33000), (1040, 32264), (1040, 32263), (2048, 16384), (2048, 16383), (4080, 8224), (4095, 8300), (4096, 8192), (4096, 5120), (4096, 5121)):
+        x, xs, w, ws, ref = product_case(m, n, k, torch.float16, pad=-k % 16)            # rows on 16 bytes
+        check_product(L.int8_matmul(x, xs, w, ws, out_dtype="f32"), ref, torch.float32)
+    status_ok()
