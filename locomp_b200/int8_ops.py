@@ -40,6 +40,8 @@ class QuantizedTokens:
 @contextmanager
 def _on(device: int, stream):
     """Work on a device and on `stream` (None: the device's current one): what is allocated in here belongs to that stream."""
+    if isinstance(stream, torch.cuda.Stream) and stream.device.index != device:          # (its context would launch on its own device)
+        raise ValueError(f"the operands live on cuda:{device}, the stream on {stream.device}")
     with torch.cuda.device(device):
         if stream is None:
             yield

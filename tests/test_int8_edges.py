@@ -2,6 +2,7 @@
 
 Bounds are those of test_int8_path.py: a product is an exact integer, three float32 roundings and the output's own; a normalised value
 is good to REL = 2^-18."""
+import contextlib
 import ctypes
 import itertools
 import os
@@ -14,7 +15,7 @@ import pytest
 import torch
 
 import locomp_b200 as L
-from locomp_b200 import _lib
+from locomp_b200 import _lib, int8_ops
 from test_int8_path import HALF_STEP, KINDS, NAMES, REL, check_product, check_tokens, gen, plan, product_case, rms, status_ok
 
 tensor_module = sys.modules["locomp_b200.tensor"]        # (the package's `tensor` is a function)
@@ -291,6 +292,22 @@ def test_batches_of_sequences(shape, n, k):
     empty = L.quantize_tokens(x[:0])
     assert layer(empty).shape == (0,) + shape[1:] + (n,)
     status_ok()
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    """Its context would make its device the current one, and the kernel would run there on this device's addresses."""
+    class Stream:
+        device, cuda_stream = torch.device("cuda", 1), 4096
+    entered = []
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    monkeypatch.setattr(torch.cuda, "device", lambda d: contextlib.nullcontext())
+    monkeypatch.setattr(torch.cuda, "stream", lambda s: contextlib.nullcontext(entered.append(s)))
+    with pytest.raises(ValueError, match="stream on cuda:1"):
+        with int8_ops._on(0, Stream()):
+            pass
+    assert not entered
+    with int8_ops._on(1, Stream()):
+        assert len(entered) == 1
 
 
 @pytest.mark.gpu
