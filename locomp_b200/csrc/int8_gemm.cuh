@@ -60,7 +60,8 @@ constexpr int BAR_ALL = 1, BAR_GROUP = 2;    // named barriers: both groups; gro
 constexpr int MAX_K = 131071;
 constexpr int MAX_SPLIT = 8;                 // CTAs of a cluster that share a tile's K
 
-// Division of 0 <= n < 2^31 by a divisor of the host's choosing: the walk's divisions by Params took 2000 clocks a tile.
+// Division of 0 <= n < 2^31 by a divisor of the host's choosing, as a product with its reciprocal (Granlund and Montgomery, Division by Invariant Integers
+// using Multiplication, 1994): the walk's divisions by Params took 2000 clocks a tile.
 struct Divisor {
   uint32_t mul;
   int shift;
@@ -426,7 +427,7 @@ int8_gemm_kernel(const __grid_constant__ CUtensorMap tmap_x, const __grid_consta
     }
   } else if (warp < N_EPI) {
     // ------------------------------------------------------------ epilogue warps: TMEM -> global
-    griddep_wait();                            // out and the scratch may still be in the preceding kernel's use
+    griddep_wait();                            // out may still be in the preceding kernel's use
     constexpr int C = chunk_columns<OT>();
     const int group = warp >> 2, in_group = warp & 3;
     const int r = in_group * 32 + lane;        // weight row of the tile = TMEM lane

@@ -125,7 +125,7 @@ def quantize_tokens(x, weight=None, eps: float = 1e-5, *, out: Optional[Quantize
     wo = None if weight is None else resolve(weight, "weight", bf16)
     if wo is not None and wo.size != n:
         raise ValueError(f"weight must hold n = {n} values, got {wo.size}")
-    kind, dev = _same(xo) if wo is None else _same(xo, wo)
+    _, dev = _same(xo) if wo is None else _same(xo, wo)
     code = _float_kind(xo, "x")
     _require_cuda()
     with _on(dev, stream):
@@ -146,7 +146,7 @@ def silu_mul_tokens(gate, up, *, out: Optional[QuantizedTokens] = None, stream=N
     if go.shape != uo.shape:
         raise ValueError(f"gate and up must have one shape, got {go.shape} and {uo.shape}")
     rows, n = _rows_of(go, "gate")
-    kind, dev = _same(go, uo)
+    _, dev = _same(go, uo)
     code = _float_kind(go, "gate")
     _require_cuda()
     with _on(dev, stream):
