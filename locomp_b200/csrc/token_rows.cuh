@@ -418,7 +418,7 @@ __global__ void __launch_bounds__(MAX_THREADS, BLOCKS) rows_kernel(const Args p)
         }
       }
       if (QUANT) {
-        store_q<ALIGNED, OP == ROWS, NORMED>(static_cast<int8_t*>(p.out) + row * p.ldo, i, n, v, s, inv, finite);
+        store_q<ALIGNED, OP == ROWS, NORMED && sizeof(T) == 2>(static_cast<int8_t*>(p.out) + row * p.ldo, i, n, v, s, inv, finite);
       } else {
         Octet<T> o;
         o.set(v);
