@@ -426,7 +426,9 @@ PyObject* residual_norms(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     return not_implemented();
   const int64_t n = h->size(-1), rows = h->numel() / n;
   const int code = float_code(h->scalar_type()), delta_code = float_code(d->scalar_type());      // (delta may be float32 beside 16 bits)
-  if (code == NOT_FLOAT || (delta_code != code && delta_code != LCQ_F32) || d->device() != h->device() || d->dim() < 1 || d->numel() != h->numel() || d->size(-1) != n || n > MOST_PER_ROW) return not_implemented();
+  if (code == NOT_FLOAT || (delta_code != code && delta_code != LCQ_F32) || d->device() != h->device() || d->dim() < 1 || d->numel() != h->numel() ||
+      d->size(-1) != n || n > MOST_PER_ROW)
+    return not_implemented();
   const at::Tensor* more[3] = {nullptr, nullptr, nullptr};        // weight, post_weight, gate
   const int where[3] = {2, 4, 5};
   for (int i = 0; i < 3; ++i) {
@@ -474,7 +476,8 @@ PyObject* int8_matmul(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   long long wanted;
   if (!x || !xs || !w || !ws || !as_int(args[5], wanted) || wanted < -1 || wanted > LCQ_BF16) return not_implemented();
   if (x->scalar_type() != at::kChar || w->scalar_type() != at::kChar || xs->scalar_type() != at::kFloat) return not_implemented();
-  if ((x->dim() > 2 && xs->sizes() != x->sizes().slice(0, x->dim() - 1)) || w->dim() != 2 || w->device() != x->device() || xs->device() != x->device() || ws->device() != x->device())
+  if ((x->dim() > 2 && xs->sizes() != x->sizes().slice(0, x->dim() - 1)) || w->dim() != 2 || w->device() != x->device() || xs->device() != x->device() ||
+      ws->device() != x->device())
     return not_implemented();
   const int64_t K = x->size(-1), M = x->numel() / K, N = w->size(0);
   constexpr int64_t most = 2000000000;
